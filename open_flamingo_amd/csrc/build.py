@@ -44,7 +44,7 @@ TOOLS_LIB = os.path.join(ROOT, "tools", "libofhip_tools.so")
 
 def build(emu=False, verbose=False, force=False, tools=False):
     srcs = [os.path.join(HERE, s) for s in SOURCES if os.path.exists(os.path.join(HERE, s)) and (emu or tools or s not in TOOLS_ONLY_SOURCES)]
-    hdrs = [h if os.path.isabs(h) else os.path.join(HERE, h) for h in HEADERS]
+    hdrs = [h if os.path.isabs(h) else os.path.join(HERE, h) for h in HEADERS] + [os.path.abspath(__file__)]      # (a change of flags rebuilds)
     if emu:
         hdrs.append(os.path.join(EMU_DIR, "of_emu.h"))
         objdir = os.path.join(EMU_DIR, "build")
@@ -55,7 +55,8 @@ def build(emu=False, verbose=False, force=False, tools=False):
     else:
         objdir = os.path.join(HERE, "build_tools" if tools else "build")
         cc = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-std=c++17", "-O3", "-fPIC", "-I", HERE,
-              "-Wno-unused-function", "-fno-fast-math"]   # erf / tanh / division semantics of the epilogues stay IEEE
+              "-Wno-unused-function", "-fno-fast-math",   # erf / tanh / division semantics of the epilogues stay IEEE
+              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]   # no v_pk_{add,mul,fma}_f32: some forms of them have returned wrong values
         if tools:
             cc.append("-DOF_TOOLS_BUILD")
         lib = TOOLS_LIB if tools else LIB
