@@ -1,0 +1,166 @@
+// Epilogues of the 256x256 GEMM kernel (gemm_w4m.hip) for the loss of a language-model head whose logits are never kept
+// (linear_ce.hip).  Four products of it run on that kernel; a wave owns 128 x 128 of a tile and sends it as eight 32 x 64 groups
+// through its LDS patch (gemm_common.h), so that in a row pass eight lanes hold 8 consecutive columns each of one row:
+//   LSE     z = s x W^T: per row and 128-column strip (max, sum exp(z - max)) -> part[strip][row]; the label's z -> zlab[row].
+//           Statistics in fp32 straight from the fp32 accumulators: a logit is never rounded to bf16.
+//   DLOGIT  the same product again: D = exp(z - lse[row]) - [column == label], times the row's upstream gradient where rows have one of
+//           their own, stored as bf16 (the operand type of the two products behind it; half a unit of 2^-8 of each entry at most).  A
+//           scalar upstream gradient is NOT in D -- it multiplies the fp32 sums of those products instead, so that -1 + p keeps its bits.
+//   DX      dx_acc (fp32) = beta dx_acc + D W over the pieces of the vocabulary
+//   DW      dW (bf16) = scale D^T x
+// Rows are the compacted ones (labels that count), padded to 256; the vocabulary's last tile hangs over the table's end: its rows
+// read as zeros (of_buf_make_n), its columns are masked here.
+#pragma once
+#include "gemm_tile256.h"
+
+enum { OF_EPI_CE_LSE = 16, OF_EPI_CE_DLOGIT = 17, OF_EPI_CE_DX = 18, OF_EPI_CE_DW = 19 };      // internal: of_gemm refuses them
+OF_HOSTDEV constexpr bool of_epi_is_ce(int epi) { return epi >= OF_EPI_CE_LSE; }
+
+struct OfCeGemmArgs : OfGemmArgs {      // M, N, K: the padded extents of the launch (of_gemm's layout rules)
+    const int* count;        // device: rows with a label that counts; live rows = count rounded up to 256, at least 256 (M, or K of DW)
+    long b_bytes;            // bytes of the B matrix from args.B to the end of its last row
+    int n_valid;             // columns that exist (LSE, DLOGIT: vocabulary of the piece; DX, DW: d)
+    int m_valid;             // DW: rows that exist (vocabulary of the piece)
+    int col0;                // vocabulary index of column 0 of the piece (labels count from the table's first row)
+    const int* lab;          // [row] label, -1 for rows behind `count`
+    const float* lse;        // [row], +inf for rows behind `count`
+    const float* grow;       // [row] upstream gradient of its own, or NULL
+    float* part;             // LSE: [strip][row][2]
+    float* zlab;             // LSE: [row]
+    long part_ld;            // rows of one strip
+    const float* gscale;     // DW: scalar upstream gradient or NULL (1)
+    int by_count;            // DW: divide by `count`
+};
+int of_gemm_w4m_ce(const OfCeGemmArgs& a, of_stream_t s);      // gemm_w4m.hip: a.epi selects the product
+
+template <int EPI>
+struct OfEpiArgs { typedef OfGemmArgs type; };
+template <> struct OfEpiArgs<OF_EPI_CE_LSE> { typedef OfCeGemmArgs type; };
+template <> struct OfEpiArgs<OF_EPI_CE_DLOGIT> { typedef OfCeGemmArgs type; };
+template <> struct OfEpiArgs<OF_EPI_CE_DX> { typedef OfCeGemmArgs type; };
+template <> struct OfEpiArgs<OF_EPI_CE_DW> { typedef OfCeGemmArgs type; };
+
+// rows a launch works on: at least one tile, so that every product, sum and gradient of a batch without a single label is written (as zeros)
+OF_HOSTDEV int of_ce_live_rows(int count) { return count > 0 ? (count + 255) & ~255 : 256; }
+// the scalar that multiplies both gradients: upstream / number of labels (mean), upstream (sum), 1 (rows have their own)
+OF_DEV float of_ce_scale(const float* gscale, int by_count, const int* count) {
+    if (by_count && *count == 0) return 0.f;
+    const float g = gscale ? *gscale : 1.0f;
+    return by_count ? g / (float)*count : g;
+}
+
+namespace oft {
+
+constexpr float CE_LOG2E = 1.4426950408889634f;
+constexpr float CE_LOWEST = -3.0e38f;      // the running maximum of nothing: below every finite logit, and no NaN in differences
+
+// the row passes of one 32 x 64 group (accumulators in the patch)
+template <int EPI>
+OF_DEV void ce_group_rows(const OfCeGemmArgs& p, char* patch, int m_base, int n_base, int lane, float sc, float (&mx)[4], float (&sm)[4]) {
+    constexpr bool SPLIT = EPI == OF_EPI_CE_DX;          // fp32 output: columns 4j.. and 32 + 4j.. (gemm_common.h, epi_split_cols)
+    const int hi = SPLIT ? 32 : 4;
+    const int rd_row = lane >> 3, rd_col = (lane & 7) * (SPLIT ? 4 : 8);
+    of_wave_sync();
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+        const int r = it * 8 + rd_row, m = m_base + r, n = n_base + rd_col;
+        const f32x4 v0 = *(const f32x4*)(patch + r * ofg::PATCH_PITCH + rd_col * 4), v1 = *(const f32x4*)(patch + r * ofg::PATCH_PITCH + (rd_col + hi) * 4);
+        float a[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+        if constexpr (EPI == OF_EPI_CE_LSE || EPI == OF_EPI_CE_DLOGIT) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a[e] *= sc;
+            const int at = p.lab[m] - p.col0 - n;         // the label's place among this lane's eight columns, if 0 <= at < 8
+            if constexpr (EPI == OF_EPI_CE_LSE) {
+                if (n + 8 > p.n_valid) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (n + e >= p.n_valid) a[e] = -__builtin_inff();
+                }
+                float top = mx[it];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = of_max(top, a[e]);
+                float s = sm[it] * of_exp2((mx[it] - top) * CE_LOG2E);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s += of_exp2((a[e] - top) * CE_LOG2E);
+                mx[it] = top;
+                sm[it] = s;
+                if ((unsigned)at < 8u && n + at < p.n_valid) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e == at) p.zlab[m] = a[e];
+                }
+            } else {
+                const float l = p.lse[m], g = p.grow ? p.grow[m] : 1.0f;
+                float o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float d = of_exp2((a[e] - l) * CE_LOG2E) - (e == at ? 1.0f : 0.0f);
+                    o[e] = n + e < p.n_valid ? g * d : 0.f;
+                }
+                *(u32x4*)((bf16_t*)p.C + (size_t)m * p.ldc + n) = ofg::pack8(o);
+            }
+        } else if constexpr (EPI == OF_EPI_CE_DX) {
+            float* c = (float*)p.C + (size_t)m * p.ldc + n;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (n + h * 32 >= p.n_valid) continue;
+                f32x4 o = {a[4 * h], a[4 * h + 1], a[4 * h + 2], a[4 * h + 3]};
+                if (p.beta != 0.f) {
+                    const f32x4 old = *(const f32x4*)(c + h * 32);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] += old[e];
+                }
+                *(f32x4*)(c + h * 32) = o;
+            }
+        } else {
+            if (m < p.m_valid && n < p.n_valid) {
+                float o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = sc * a[e];
+                *(u32x4*)((bf16_t*)p.C + (size_t)m * p.ldc + n) = ofg::pack8(o);
+            }
+        }
+        of_sched_fence();
+    }
+    of_wave_sync();
+}
+
+template <int EPI, class ToPatch>
+OF_DEV void w4_epilogue_ce(const OfCeGemmArgs& p, ToPatch to_patch, char* smem, int m0, int n0, int wm, int wn, int wave, int lane) {
+    char* patch = smem + wave * ofg::PATCH_BYTES;
+    float sc = p.alpha;
+    if (EPI == OF_EPI_CE_DW) sc *= of_ce_scale(p.gscale, p.by_count, p.count);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+        float mx[4], sm[4];
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            mx[it] = CE_LOWEST;
+            sm[it] = 0.f;
+        }
+#pragma unroll
+        for (int np = 0; np < 2; ++np) {
+            to_patch(2 * mt + np, patch);
+            ce_group_rows<EPI>(p, patch, m0 + wm * 128 + mt * 32, n0 + wn * 128 + np * 64, lane, sc, mx, sm);
+        }
+        if constexpr (EPI == OF_EPI_CE_LSE) {          // the strip's 128 columns sit in eight lanes: join them, one (max, sum) per row
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+#pragma unroll
+                for (int o = 4; o >= 1; o >>= 1) {
+                    const float m2 = of_shfl_xor(mx[it], o), s2 = of_shfl_xor(sm[it], o);
+                    const float top = of_max(mx[it], m2);
+                    sm[it] = sm[it] * of_exp2((mx[it] - top) * CE_LOG2E) + s2 * of_exp2((m2 - top) * CE_LOG2E);
+                    mx[it] = top;
+                }
+                if ((lane & 7) == 0) {
+                    const size_t strip = (size_t)(n0 >> 7) + wn;
+                    const int m = m0 + wm * 128 + mt * 32 + it * 8 + (lane >> 3);
+                    *(f32x2*)(p.part + (strip * p.part_ld + m) * 2) = f32x2{mx[it], sm[it]};
+                }
+            }
+        }
+    }
+}
+
+}  // namespace oft

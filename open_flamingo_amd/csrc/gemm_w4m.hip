@@ -30,6 +30,7 @@
 #include <type_traits>
 #include "gemm_tile256.h"
 #include "gemm_w4_epi.h"
+#include "gemm_ce_epi.h"
 
 // K rotation of a tile's stage loop (see the kernel): the workgroups of XCD x (block id & 7) start at stage x * (stages / 8).  The 32
 // tiles an XCD runs at a time share A and B panels through its L2 and must walk K together; the eight XCDs need not -- measured on
@@ -114,7 +115,7 @@ struct W4M_B3 {
 #ifdef OF_W4M_NO_B3          // tools/ab builds only: the other arm of the same-box A/B
     static constexpr bool value = false;
 #else
-    static constexpr bool value = EPI == OF_EPI_STORE_BF16 || EPI == OF_EPI_GELU || EPI == OF_EPI_ACC_F32 || (EPI == OF_EPI_GATE_RESID && W4M_B3_RESID);
+    static constexpr bool value = EPI == OF_EPI_STORE_BF16 || EPI == OF_EPI_GELU || EPI == OF_EPI_ACC_F32 || (EPI == OF_EPI_GATE_RESID && W4M_B3_RESID) || of_epi_is_ce(EPI);
 #endif
 };
 
@@ -135,10 +136,20 @@ OF_HOSTDEV size_t sk_dot_bytes(const OfGemmArgs& a) { return of_gemm_dot_bytes(a
 // wait late and only for workgroups with LOWER ids: no deadlock even when fewer than G workgroups are resident (the hardware
 // dispatches in id order; a workgroup's first segment never waits).  The owner adds the partials in ascending K order, on top
 // of its own: the same bits for the same (shape, G), whatever the timing.
+// The epilogues of a vocabulary head's loss (gemm_ce_epi.h) run classic launches only; their row count is on the device: M (K of the weight
+// gradient) is what the rows with a label fill, workgroups without a tile leave at once.
 // SK = false: the classic launch compiled on its own -- one tile per workgroup, none of the schedule arithmetic, flags or partial
 // tile code (as one kernel the bookkeeping cost every tile of every launch 0.7-1 us of prologue: profiles/r04g_tile_phase_probe.jsonl).
 template <bool AT, bool BT, int EPI, bool SK>
-OF_GLOBAL void OF_BOUNDS(256, 1) of_gemm_w4m_kernel(OfGemmArgs p) {
+OF_GLOBAL void OF_BOUNDS(256, 1) of_gemm_w4m_kernel(typename OfEpiArgs<EPI>::type p) {
+    constexpr bool CE = of_epi_is_ce(EPI);
+    static_assert(!CE || !SK, "classic launches only");
+    if constexpr (CE) {
+        const int live = of_ce_live_rows(of_uniform(*p.count));
+        if (EPI == OF_EPI_CE_DW) p.K = live;
+        else p.M = live;
+        if (of_bid_x() >= (p.M / TM) * (p.N / TN)) return;          // (the whole workgroup, in front of every barrier)
+    }
     constexpr bool ASMD = AT || BT;       // LDS-DMA form (of_platform.h): inline asm wherever a transposed-fragment read follows
     OF_STAMP_DECL();
     OF_STAMP(0);
@@ -148,7 +159,7 @@ OF_GLOBAL void OF_BOUNDS(256, 1) of_gemm_w4m_kernel(OfGemmArgs p) {
     const int wm = wave >> 1, wn = wave & 1;
     const int tiles_m = p.M / TM, tiles_n = p.N / TN, ntiles = tiles_m * tiles_n;
     const int nd_all = p.K / DK;
-    const int G = of_gdim_x(), bid = of_bid_x();
+    const int G = CE ? ntiles : of_gdim_x(), bid = of_bid_x();
     // (32-bit arithmetic: r * nd * G < 2^31 for every K < 2 M; the classic launch skips the divisions altogether -- a 64-bit
     // division is ~150 instructions, and this code sits in front of every tile)
     int rounds = 1;
@@ -225,7 +236,14 @@ OF_GLOBAL void OF_BOUNDS(256, 1) of_gemm_w4m_kernel(OfGemmArgs p) {
             Bmat = (const bf16_t*)of_uniform_ptr(p.groups[grp]);      // loaded behind the previous segment's stores: a vector load
             nB = n0 - grp * p.group_extent;
         }
-        const of_buf_t gB = of_buf_make(chunk_base<BT>(Bmat, p.ldb, nB));
+        of_buf_t gB;
+        if constexpr (CE) {          // B ends where its matrix ends: what the last tile or K stage reads behind it arrives as zeros
+            const bf16_t* at = chunk_base<BT>(Bmat, p.ldb, nB);
+            const long left = p.b_bytes - (long)((const char*)at - (const char*)Bmat);
+            gB = of_buf_make_n(at, left < 0xffffffffl ? (unsigned)left : 0xffffffffu);
+        } else {
+            gB = of_buf_make(chunk_base<BT>(Bmat, p.ldb, nB));
+        }
         // K rotation: a workgroup that holds ALL K stages of its tile starts at stage `rot` and wraps around (same products, another
         // order of the fp32 additions).  Without it every workgroup of the launch reads K offset 64 d of its panels at the same time;
         // with a power-of-two row pitch those addresses differ in high bits only and land on the same few HBM channels.
@@ -426,7 +444,8 @@ OF_GLOBAL void OF_BOUNDS(256, 1) of_gemm_w4m_kernel(OfGemmArgs p) {
             }
         };
         // gate-gradient partial of this TILE: slot = its position in the (m-major) tile grid, whichever workgroup finishes it
-        w4_epilogue_with<EPI, ASMD, decltype(acc_to_patch), true, !(EPI == OF_EPI_GATE_RESID && B3)>(p, acc_to_patch, smem, SMEM_W4M, m0, n0, wm, wn, wave, lane, pm * tiles_n + pn);
+        if constexpr (CE) w4_epilogue_ce<EPI>(p, acc_to_patch, smem, m0, n0, wm, wn, wave, lane);
+        else w4_epilogue_with<EPI, ASMD, decltype(acc_to_patch), true, !(EPI == OF_EPI_GATE_RESID && B3)>(p, acc_to_patch, smem, SMEM_W4M, m0, n0, wm, wn, wave, lane, pm * tiles_n + pn);
         OF_STAMP(3);
     }
     OF_STAMP_FLUSH();
@@ -479,6 +498,24 @@ size_t of_gemm_w4m_sk_bytes(const OfGemmArgs& a, int grid) {
     const int ntiles = (a.M / TM) * (a.N / TN);
     if (grid <= 0 || ntiles % grid == 0) return 0;
     return sk_dot_bytes(a) + sk_flags_bytes(grid) + (size_t)grid * SK_SLAB_BYTES;
+}
+
+// The products of linear_ce.hip (declared in gemm_ce_epi.h): M, N multiples of 256, K of 64, grid for every row of the batch; the caller
+// guarantees that A holds M x K (K x M) elements and that the spans below fit 32-bit byte offsets.
+int of_gemm_w4m_ce(const OfCeGemmArgs& a, of_stream_t s) {
+    if ((a.M % TM) || (a.N % TN) || (a.K % DK) || a.M <= 0 || a.N <= 0 || a.K <= 0 || a.b_bytes <= 0) return OF_E_SHAPE;
+    const unsigned long long a_span = 2ull * (unsigned long long)(a.a_trans ? a.K : TM) * (unsigned long long)a.lda;
+    const unsigned long long b_span = 2ull * (unsigned long long)(a.b_trans ? a.K : TN) * (unsigned long long)a.ldb;
+    if (a_span >= (1ull << 32) || b_span >= (1ull << 32)) return OF_E_SHAPE;
+    const of_dim3 grid{(unsigned)((a.M / TM) * (a.N / TN)), 1, 1};
+    constexpr int smem = SMEM_W4M + OPER_BYTES;
+    switch (a.epi) {
+        case OF_EPI_CE_LSE: return of_launch(of_gemm_w4m_kernel<false, false, OF_EPI_CE_LSE, false>, grid, 256, smem, s, a);
+        case OF_EPI_CE_DLOGIT: return of_launch(of_gemm_w4m_kernel<false, false, OF_EPI_CE_DLOGIT, false>, grid, 256, smem, s, a);
+        case OF_EPI_CE_DX: return of_launch(of_gemm_w4m_kernel<false, true, OF_EPI_CE_DX, false>, grid, 256, smem, s, a);
+        case OF_EPI_CE_DW: return of_launch(of_gemm_w4m_kernel<true, true, OF_EPI_CE_DW, false>, grid, 256, smem, s, a);
+    }
+    return OF_E_ARG;
 }
 
 int of_gemm_w4m_try(const OfGemmArgs& a, of_stream_t s) {

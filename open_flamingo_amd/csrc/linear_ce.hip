@@ -1,0 +1,384 @@
+// Softmax cross entropy of a language-model head whose logits are never kept (gfx950):  z = s x W^T over a vocabulary of ~50 000,
+// loss_r = log sum_v exp z_rv - z_r,label, and its gradients dx = s g D W, dW = s g D^T x with D = softmax(z) - onehot(label).
+//
+// Materialised (loss.hip behind a vendor GEMM) the logits of 8192 rows are 826 MB in bf16, written once and read twice, and rounded
+// to 8 bits of mantissa in front of the exponential.  Here:
+//   forward   rows whose label counts are gathered (an ignored row costs nothing behind this point), then ONE product whose epilogue
+//             keeps (max, sum exp) per row and 128 columns, from fp32 accumulators; a small launch joins the ~400 strips of a row;
+//   backward  the vocabulary in pieces: the product again -> D of the piece (bf16, at most a few hundred MB, sized so that it stays in
+//             the 256-MB Infinity Cache between the three products that touch it) -> dx += D W_piece in fp32, dW_piece = D^T x.
+// All products run on the 256x256 MFMA kernel (gemm_w4m.hip) with the epilogues of gemm_ce_epi.h: they are bound by its K loop, i.e. by
+// the chip's power budget, 2 R V d operations forward and 6 R V d backward (a third of them the second logits product).
+// No atomics; every sum has a fixed order.
+#include "gemm_ce_epi.h"
+
+namespace {
+
+constexpr int CE_THREADS = 512;
+
+struct CeRowsArgs {
+    const long long* labels; long long ignore_index;
+    long rows; int vocab;
+    int* count; int* slot_of; int* row_of; int* lab;
+    float* lse; float* loss_rows;
+    const bf16_t* x; long ldx; bf16_t* xc; long ldxc; int d, d_pad;
+    const float* part; const float* zlab; long part_ld; int strips;
+    float* loss; int mean;
+    const float* grad; int by_count; float logit_scale; const float* acc; long ldacc; bf16_t* dx; long lddx;
+    float* grow;
+    const bf16_t* w; long ldw; bf16_t* wc; long ldwc; long w_rows;
+};
+
+// One workgroup: the rows whose label counts, in order.  slot_of[row] = place among them or -1, row_of its inverse, lab by place;
+// loss_rows of the others is final here: 0 for ignored rows, NaN for a label outside the vocabulary (a caller's mistake that has to
+// surface in the loss; such a row has no gradient).
+OF_GLOBAL void OF_BOUNDS(CE_THREADS, 1) ce_index_kernel(CeRowsArgs a) {
+    int* cum = (int*)of_smem();
+    const int tid = of_tid();
+    const long per = (a.rows + CE_THREADS - 1) / CE_THREADS, lo = tid * per, hi = lo + per < a.rows ? lo + per : a.rows;
+    int n = 0;
+    for (long r = lo; r < hi; ++r) {
+        const long long l = a.labels[r];
+        n += l != a.ignore_index && l >= 0 && l < a.vocab;
+    }
+    cum[tid] = n;
+    of_sync();
+    for (int o = 1; o < CE_THREADS; o <<= 1) {
+        const int v = tid >= o ? cum[tid - o] : 0;
+        of_sync();
+        cum[tid] += v;
+        of_sync();
+    }
+    int at = cum[tid] - n;
+    for (long r = lo; r < hi; ++r) {
+        const long long l = a.labels[r];
+        const bool counts = l != a.ignore_index && l >= 0 && l < a.vocab;
+        a.slot_of[r] = counts ? at : -1;
+        if (counts) {
+            a.row_of[at] = (int)r;
+            a.lab[at] = (int)l;
+            ++at;
+        } else {
+            a.loss_rows[r] = l == a.ignore_index ? 0.f : __builtin_nanf("");
+        }
+    }
+    const int total = cum[CE_THREADS - 1];
+    if (tid == 0) *a.count = total;
+    for (int i = total + tid; i < of_ce_live_rows(total); i += CE_THREADS) a.lab[i] = -1;
+}
+
+// xc[place] = x[row_of[place]], zeros in the columns behind d and in the rows behind `count` up to the next 256: the products then
+// need no row or depth edges.  One wave per row.
+OF_GLOBAL void OF_BOUNDS(256, 4) ce_gather_kernel(CeRowsArgs a) {
+    const int lane = of_tid() & 63, count = *a.count;
+    const long i = (long)of_bid_x() * 4 + (of_tid() >> 6);
+    if (i >= of_ce_live_rows(count)) return;
+    const bf16_t* src = i < count ? a.x + (size_t)a.row_of[i] * a.ldx : nullptr;
+    bf16_t* dst = a.xc + (size_t)i * a.ldxc;
+    for (int c = lane * 8; c < a.d_pad; c += 512) {
+        u32x4 v = {0u, 0u, 0u, 0u};
+        if (src && c < a.d) v = *(const u32x4*)(src + c);
+        *(u32x4*)(dst + c) = v;
+    }
+}
+
+// the table with its rows padded to a multiple of 64 columns by zeros (only where d is none)
+OF_GLOBAL void OF_BOUNDS(256, 4) ce_pad_table_kernel(CeRowsArgs a) {
+    const int lane = of_tid() & 63;
+    for (long i = (long)of_bid_x() * 4 + (of_tid() >> 6); i < a.w_rows; i += (long)of_gdim_x() * 4)
+        for (int c = lane * 8; c < a.d_pad; c += 512) {
+            u32x4 v = {0u, 0u, 0u, 0u};
+            if (c < a.d) v = *(const u32x4*)(a.w + (size_t)i * a.ldw + c);
+            *(u32x4*)(a.wc + (size_t)i * a.ldwc + c) = v;
+        }
+}
+
+// 16 rows a workgroup, 16 lanes a row: lane j joins strips j, j + 16, ... of its row, then the 16 lanes in a fixed order
+OF_GLOBAL void OF_BOUNDS(256, 2) ce_finish_kernel(CeRowsArgs a) {
+    float* red = (float*)of_smem();          // [16 groups][16 rows][2]
+    const int tid = of_tid(), r = tid & 15, j = tid >> 4, count = *a.count;
+    const long i0 = (long)of_bid_x() * 16;
+    if (i0 >= of_ce_live_rows(count)) return;
+    const long i = i0 + r;
+    float m = oft::CE_LOWEST, s = 0.f;
+    for (int t = j; t < a.strips; t += 16) {
+        const f32x2 q = *(const f32x2*)(a.part + ((size_t)t * a.part_ld + i) * 2);
+        const float top = of_max(m, q[0]);
+        s = s * of_exp2((m - top) * oft::CE_LOG2E) + q[1] * of_exp2((q[0] - top) * oft::CE_LOG2E);
+        m = top;
+    }
+    red[(j * 16 + r) * 2] = m;
+    red[(j * 16 + r) * 2 + 1] = s;
+    of_sync();
+    if (j == 0) {
+        float top = red[r * 2];
+        for (int k = 1; k < 16; ++k) top = of_max(top, red[(k * 16 + r) * 2]);
+        float sum = 0.f;
+        for (int k = 0; k < 16; ++k) sum += red[(k * 16 + r) * 2 + 1] * of_exp2((red[(k * 16 + r) * 2] - top) * oft::CE_LOG2E);
+        const float lse = top + of_log2(sum) * 0.69314718055994531f;
+        a.lse[i] = i < count ? lse : __builtin_inff();          // behind `count`: exp(z - inf) = 0, rows of D that are zero
+        if (i < count) a.loss_rows[a.row_of[i]] = lse - a.zlab[i];
+    }
+}
+
+// one workgroup: the sum of the rows' losses, divided by the number of labels for a mean (0 / 0 = NaN without any, as torch has it)
+OF_GLOBAL void OF_BOUNDS(CE_THREADS, 1) ce_reduce_kernel(CeRowsArgs a) {
+    float* red = (float*)of_smem();
+    const int tid = of_tid();
+    float s = 0.f;
+    for (long r = tid; r < a.rows; r += CE_THREADS) s += a.loss_rows[r];
+    red[tid] = s;
+    of_sync();
+    for (int o = CE_THREADS / 2; o >= 1; o >>= 1) {
+        if (tid < o) red[tid] += red[tid + o];
+        of_sync();
+    }
+    if (tid == 0) *a.loss = a.mean ? red[0] / (float)*a.count : red[0];
+}
+
+// upstream gradients of the rows, by place
+OF_GLOBAL void OF_BOUNDS(256, 4) ce_row_grads_kernel(CeRowsArgs a) {
+    const long i = (long)of_bid_x() * 256 + of_tid();
+    const int count = *a.count;
+    if (i < of_ce_live_rows(count)) a.grow[i] = i < count ? a.grad[a.row_of[i]] : 0.f;
+}
+
+// dx[row] = bf16(logit_scale * scale * acc[place]), zeros for rows without a label; one wave per row
+OF_GLOBAL void OF_BOUNDS(256, 4) ce_scatter_kernel(CeRowsArgs a) {
+    const int lane = of_tid() & 63;
+    const long r = (long)of_bid_x() * 4 + (of_tid() >> 6);
+    if (r >= a.rows) return;
+    const int i = a.slot_of[r];
+    const float sc = a.logit_scale * of_ce_scale(a.grad, a.by_count, a.count);
+    const float* src = i < 0 ? nullptr : a.acc + (size_t)i * a.ldacc;
+    bf16_t* dst = a.dx + (size_t)r * a.lddx;
+    for (int c = lane * 8; c < a.d; c += 512) {
+        float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (src) {
+            const f32x4 v0 = *(const f32x4*)(src + c), v1 = *(const f32x4*)(src + c + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[e] = sc * v0[e];
+                o[4 + e] = sc * v1[e];
+            }
+        }
+        *(u32x4*)(dst + c) = ofg::pack8(o);
+    }
+}
+
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+long rows_padded(long rows) { return rows > 0 ? (rows + 255) & ~255l : 256; }
+int depth_padded(int d) { return (d + 63) & ~63; }
+
+// what the forward leaves for the backward
+struct CeState {
+    int *count, *slot_of, *row_of, *lab;
+    float* lse;
+    bf16_t* xc;
+    size_t bytes;
+};
+CeState ce_state(void* base, long rows, int d) {
+    const size_t rp = (size_t)rows_padded(rows);
+    char* at = (char*)base;
+    CeState s{};
+    auto take = [&](size_t n) {
+        char* p = at;
+        at += up256(n);
+        return p;
+    };
+    s.count = (int*)take(4);
+    s.slot_of = (int*)take(rp * 4);
+    s.row_of = (int*)take(rp * 4);
+    s.lab = (int*)take(rp * 4);
+    s.lse = (float*)take(rp * 4);
+    s.xc = (bf16_t*)take(rp * depth_padded(d) * 2);
+    s.bytes = (size_t)(at - (char*)base);
+    return s;
+}
+
+// Vocabulary rows of one backward piece.  D (rows x piece, bf16) is written once and read twice: up to 128 MB it stays in the Infinity
+// Cache; a larger piece saves passes over the fp32 sums of dx.
+int ce_piece(const OfLinearCeArgs& a) {
+    long p = a.piece;
+    if (p <= 0) p = (128l << 20) / (2 * rows_padded(a.rows));
+    p &= ~255l;
+    const long all = (a.vocab + 255l) & ~255l;
+    if (p < 256) p = 256;
+    return (int)(p < all ? p : all);
+}
+size_t ce_table_bytes(const OfLinearCeArgs& a) { return depth_padded(a.d) != a.d ? up256((size_t)a.vocab * depth_padded(a.d) * 2) : 0; }
+
+int ce_check(const OfLinearCeArgs* args) {
+    if (!args) return OF_E_ARG;
+    const OfLinearCeArgs& a = *args;
+    if (!a.x || !a.w || !a.labels || !a.state || !a.workspace) return OF_E_ARG;
+    if (a.rows <= 0 || a.vocab <= 0 || a.d <= 0 || a.ldx < a.d || a.ldw < a.d || a.piece < 0) return OF_E_ARG;
+    if (a.reduction < OF_CE_NONE || a.reduction > OF_CE_SUM) return OF_E_ARG;
+    if ((a.d & 7) || a.rows > (1l << 30) || a.vocab > (1 << 30)) return OF_E_SHAPE;
+    if ((a.ldx & 7) || (a.ldw & 7) || ((uintptr_t)a.x & 15) || ((uintptr_t)a.w & 15) || ((uintptr_t)a.state & 15) || ((uintptr_t)a.workspace & 15))
+        return OF_E_ALIGN;
+    if (a.state_bytes < of_linear_ce_state_bytes(a.rows, a.d)) return OF_E_WORKSPACE;
+    // byte offsets inside a tile's operand windows are 32-bit (gemm_w4m.hip); the weight gradient walks all rows of D and of xc
+    const unsigned long long lim = 1ull << 32;
+    if (2ull * 256 * (unsigned long long)a.ldw >= lim || 2ull * (unsigned long long)rows_padded(a.rows) * depth_padded(a.d) >= lim) return OF_E_SHAPE;
+    return 0;
+}
+
+// the table the products read: the caller's, or its copy with padded rows at the start of the workspace
+int ce_table(const OfLinearCeArgs& a, of_stream_t s, const bf16_t*& w, long& ldw, char*& ws) {
+    w = a.w;
+    ldw = a.ldw;
+    ws = (char*)a.workspace;
+    if (depth_padded(a.d) == a.d) return 0;
+    CeRowsArgs r{};
+    r.w = a.w; r.ldw = a.ldw; r.w_rows = a.vocab; r.d = a.d; r.d_pad = depth_padded(a.d);
+    r.wc = (bf16_t*)ws; r.ldwc = r.d_pad;
+    w = r.wc;
+    ldw = r.ldwc;
+    ws += ce_table_bytes(a);
+    const long wg = (a.vocab + 3l) / 4;
+    return of_launch(ce_pad_table_kernel, of_dim3{(unsigned)(wg < 4096 ? wg : 4096), 1, 1}, 256, 0, s, r);
+}
+
+// the logits product of table rows [v0, v0 + n): A = the gathered rows, B = the table
+OfCeGemmArgs ce_logits_args(const OfLinearCeArgs& a, const CeState& st, const bf16_t* w, long ldw, int v0, int n) {
+    OfCeGemmArgs g{};
+    const int dp = depth_padded(a.d);
+    g.A = st.xc; g.lda = dp;
+    g.B = w + (size_t)v0 * ldw; g.ldb = (int)ldw;
+    g.M = (int)rows_padded(a.rows); g.N = (n + 255) & ~255; g.K = dp;
+    g.alpha = a.logit_scale;
+    g.count = st.count;
+    g.b_bytes = ((long)(n - 1) * ldw + dp) * 2;
+    g.n_valid = n; g.col0 = v0;
+    g.lab = st.lab; g.lse = st.lse;
+    return g;
+}
+
+}  // namespace
+
+extern "C" size_t of_linear_ce_state_bytes(long rows, int d) { return rows > 0 && d > 0 ? ce_state(nullptr, rows, d).bytes : 0; }
+
+extern "C" size_t of_linear_ce_workspace_bytes(const OfLinearCeArgs* args, int backward) {
+    if (!args || args->rows <= 0 || args->vocab <= 0 || args->d <= 0) return 0;
+    const OfLinearCeArgs& a = *args;
+    const size_t rp = (size_t)rows_padded(a.rows);
+    if (!backward) return ce_table_bytes(a) + up256((size_t)(((a.vocab + 255l) / 256) * 2) * rp * 8) + up256(rp * 4);
+    return ce_table_bytes(a) + up256(rp * (size_t)ce_piece(a) * 2) + (a.dx ? up256(rp * (size_t)a.d * 4) : 0) + (a.reduction == OF_CE_NONE ? up256(rp * 4) : 0);
+}
+
+extern "C" int of_linear_ce_fwd(const OfLinearCeArgs* args, void* stream) {
+    const int bad = ce_check(args);
+    if (bad) return bad;
+    const OfLinearCeArgs& a = *args;
+    if (!a.loss_rows || (a.reduction != OF_CE_NONE && !a.loss)) return OF_E_ARG;
+    if (a.workspace_bytes < of_linear_ce_workspace_bytes(args, 0)) return OF_E_WORKSPACE;
+    of_stream_t s = (of_stream_t)stream;
+    const CeState st = ce_state(a.state, a.rows, a.d);
+    const long rp = rows_padded(a.rows);
+    const bf16_t* w;
+    long ldw;
+    char* ws;
+    int rc = ce_table(a, s, w, ldw, ws);
+    if (rc) return rc;
+
+    CeRowsArgs r{};
+    r.labels = a.labels; r.ignore_index = a.ignore_index; r.rows = a.rows; r.vocab = a.vocab;
+    r.count = st.count; r.slot_of = st.slot_of; r.row_of = st.row_of; r.lab = st.lab; r.lse = st.lse;
+    r.loss_rows = a.loss_rows; r.loss = a.loss; r.mean = a.reduction == OF_CE_MEAN;
+    r.x = a.x; r.ldx = a.ldx; r.xc = st.xc; r.ldxc = depth_padded(a.d); r.d = a.d; r.d_pad = depth_padded(a.d);
+    rc = of_launch(ce_index_kernel, of_dim3{1, 1, 1}, CE_THREADS, CE_THREADS * sizeof(int), s, r);
+    if (rc) return rc;
+    rc = of_launch(ce_gather_kernel, of_dim3{(unsigned)(rp / 4), 1, 1}, 256, 0, s, r);
+    if (rc) return rc;
+
+    OfCeGemmArgs g = ce_logits_args(a, st, w, ldw, 0, a.vocab);
+    g.epi = OF_EPI_CE_LSE;
+    g.part = (float*)ws; g.part_ld = rp;
+    r.strips = g.N / 128;
+    g.zlab = (float*)(ws + up256((size_t)r.strips * rp * 8));
+    rc = of_gemm_w4m_ce(g, s);
+    if (rc) return rc;
+    r.part = g.part; r.part_ld = rp; r.zlab = g.zlab;
+    rc = of_launch(ce_finish_kernel, of_dim3{(unsigned)(rp / 16), 1, 1}, 256, 16 * 16 * 2 * sizeof(float), s, r);
+    if (rc || a.reduction == OF_CE_NONE) return rc;
+    return of_launch(ce_reduce_kernel, of_dim3{1, 1, 1}, CE_THREADS, CE_THREADS * sizeof(float), s, r);
+}
+
+extern "C" int of_linear_ce_bwd(const OfLinearCeArgs* args, void* stream) {
+    const int bad = ce_check(args);
+    if (bad) return bad;
+    const OfLinearCeArgs& a = *args;
+    if (!a.grad || (!a.dx && !a.dw)) return OF_E_ARG;
+    if ((a.dx && a.lddx < a.d) || (a.dw && a.lddw < a.d)) return OF_E_ARG;
+    if ((a.lddx & 7) || (a.lddw & 7) || ((uintptr_t)a.dx & 15) || ((uintptr_t)a.dw & 15)) return OF_E_ALIGN;
+    if (a.workspace_bytes < of_linear_ce_workspace_bytes(args, 1)) return OF_E_WORKSPACE;
+    of_stream_t s = (of_stream_t)stream;
+    const CeState st = ce_state(a.state, a.rows, a.d);
+    const long rp = rows_padded(a.rows);
+    const int piece = ce_piece(a), dp = depth_padded(a.d), d256 = (a.d + 255) & ~255;
+    // every operand window of the pieces' products is checked before the first launch
+    if (2ull * (unsigned long long)rp * piece >= (1ull << 32) || 2ull * (unsigned long long)piece * (unsigned long long)a.ldw >= (1ull << 32)) return OF_E_SHAPE;
+    const bf16_t* w;
+    long ldw;
+    char* ws;
+    int rc = ce_table(a, s, w, ldw, ws);
+    if (rc) return rc;
+    bf16_t* D = (bf16_t*)ws;
+    ws += up256((size_t)rp * piece * 2);
+    float* acc = nullptr;
+    if (a.dx) {
+        acc = (float*)ws;
+        ws += up256((size_t)rp * a.d * 4);
+    }
+
+    CeRowsArgs r{};
+    r.rows = a.rows; r.count = st.count; r.slot_of = st.slot_of; r.row_of = st.row_of;
+    r.d = a.d; r.acc = acc; r.ldacc = a.d; r.dx = a.dx; r.lddx = a.lddx;
+    if (a.reduction == OF_CE_NONE) {
+        r.grad = a.grad;
+        r.grow = (float*)ws;
+        rc = of_launch(ce_row_grads_kernel, of_dim3{(unsigned)((rp + 255) / 256), 1, 1}, 256, 0, s, r);
+        if (rc) return rc;
+    }
+    const float* gscale = a.reduction == OF_CE_NONE ? nullptr : a.grad;
+    const int by_count = a.reduction == OF_CE_MEAN;
+
+    for (int v0 = 0; v0 < a.vocab; v0 += piece) {
+        const int n = a.vocab - v0 < piece ? a.vocab - v0 : piece;
+        OfCeGemmArgs g = ce_logits_args(a, st, w, ldw, v0, n);
+        g.epi = OF_EPI_CE_DLOGIT;
+        g.C = D; g.ldc = piece; g.grow = r.grow;
+        rc = of_gemm_w4m_ce(g, s);
+        if (rc) return rc;
+        if (a.dx) {
+            OfCeGemmArgs q{};
+            q.epi = OF_EPI_CE_DX;
+            q.A = D; q.lda = piece;
+            q.B = w + (size_t)v0 * ldw; q.ldb = (int)ldw; q.b_trans = 1;
+            q.b_bytes = ((long)(n - 1) * ldw + dp) * 2;
+            q.M = (int)rp; q.N = d256; q.K = (n + 63) & ~63;
+            q.C = acc; q.ldc = a.d; q.beta = v0 ? 1.f : 0.f; q.alpha = 1.f;
+            q.count = st.count; q.n_valid = a.d;
+            rc = of_gemm_w4m_ce(q, s);
+            if (rc) return rc;
+        }
+        if (a.dw) {
+            OfCeGemmArgs q{};
+            q.epi = OF_EPI_CE_DW;
+            q.A = D; q.lda = piece; q.a_trans = 1;
+            q.B = st.xc; q.ldb = dp; q.b_trans = 1;
+            q.b_bytes = rp * dp * 2;
+            q.M = (n + 255) & ~255; q.N = d256; q.K = (int)rp;
+            q.C = a.dw + (size_t)v0 * a.lddw; q.ldc = (int)a.lddw;
+            q.alpha = a.logit_scale;
+            q.count = st.count; q.n_valid = a.d; q.m_valid = n;
+            q.gscale = gscale; q.by_count = by_count;
+            rc = of_gemm_w4m_ce(q, s);
+            if (rc) return rc;
+        }
+    }
+    if (!a.dx) return 0;
+    r.grad = gscale; r.by_count = by_count; r.logit_scale = a.logit_scale;
+    return of_launch(ce_scatter_kernel, of_dim3{(unsigned)((a.rows + 3) / 4), 1, 1}, 256, 0, s, r);
+}

@@ -257,6 +257,13 @@ OF_DEV of_buf_t of_buf_make(const void* base) {
     return of_buf_t{__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0xffffffff, 0x00020000),
                     u32x4{(unsigned)a, (unsigned)(a >> 32) & 0xffffu, 0xffffffffu, 0x00020000u}};
 }
+// ... of `bytes` bytes: the hardware's range check makes loads at or behind base + bytes return zeros -- also an LDS-DMA, which then
+// writes the zeros -- so that a tile may hang over the end of a matrix.  voff + soff of an access counts, soff alone must be < bytes.
+OF_DEV of_buf_t of_buf_make_n(const void* base, unsigned bytes) {
+    const unsigned long long a = (unsigned long long)base;
+    return of_buf_t{__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000),
+                    u32x4{(unsigned)a, (unsigned)(a >> 32) & 0xffffu, bytes, 0x00020000u}};
+}
 OF_DEV u32x4 of_buf_load16(of_buf_t b, unsigned voff, unsigned soff) {
     return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b.r, (int)voff, (int)soff, 0));
 }

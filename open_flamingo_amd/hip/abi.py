@@ -5,7 +5,7 @@ Pure declarations: nothing here loads a library.  ``open_flamingo_amd.hip.lib`` 
 """
 import ctypes as C
 
-OF_ABI_VERSION = 11
+OF_ABI_VERSION = 12
 OF_SUMSQ_PARTS = 512
 EPI_STORE_BF16, EPI_GELU, EPI_GATE_RESID, EPI_DGELU_DOT, EPI_SCALE_DOT, EPI_ACC_F32 = range(6)
 
@@ -78,6 +78,29 @@ class OfPackDesc(C.Structure):
     _fields_ = [("W", vp), ("P", vp), ("N", C.c_int), ("K", C.c_int), ("ldw", C.c_long)]
 
 
+CE_NONE, CE_MEAN, CE_SUM = 0, 1, 2
+
+
+class OfLinearCeArgs(C.Structure):
+    _fields_ = [
+        ("x", vp), ("ldx", C.c_long),
+        ("w", vp), ("ldw", C.c_long),
+        ("labels", vp), ("ignore_index", C.c_longlong),
+        ("rows", C.c_long),
+        ("vocab", C.c_int), ("d", C.c_int),
+        ("logit_scale", C.c_float),
+        ("reduction", C.c_int),
+        ("loss_rows", vp),
+        ("loss", vp),
+        ("state", vp), ("state_bytes", C.c_size_t),
+        ("grad", vp),
+        ("dx", vp), ("lddx", C.c_long),
+        ("dw", vp), ("lddw", C.c_long),
+        ("piece", C.c_int),
+        ("workspace", vp), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 PROTOTYPES = {
     "of_abi_version": (C.c_int, []),
     "of_build_kind": (C.c_int, []),
@@ -125,6 +148,10 @@ PROTOTYPES = {
     "of_add_embs": (C.c_int, [vp, C.c_int, vp, C.c_long, C.c_int, vp, C.c_long, C.c_int, vp, C.c_long, C.c_int, vp]),
     "of_ce_fwd": (C.c_int, [vp, C.c_int, C.c_long, vp, C.c_longlong, C.c_long, C.c_int, vp, vp, vp]),
     "of_ce_bwd": (C.c_int, [vp, C.c_int, C.c_long, vp, C.c_longlong, C.c_long, C.c_int, vp, vp, vp, C.c_long, vp]),
+    "of_linear_ce_state_bytes": (C.c_size_t, [C.c_long, C.c_int]),
+    "of_linear_ce_workspace_bytes": (C.c_size_t, [C.POINTER(OfLinearCeArgs), C.c_int]),
+    "of_linear_ce_fwd": (C.c_int, [C.POINTER(OfLinearCeArgs), vp]),
+    "of_linear_ce_bwd": (C.c_int, [C.POINTER(OfLinearCeArgs), vp]),
     "of_reduce_rows_strided": (C.c_int, [vp, C.c_int, C.c_long, C.c_int, C.c_long, C.c_int, vp, vp]),
 }
 

@@ -1,0 +1,95 @@
+"""The two ends of a language model on its vocabulary table, for training the whole table: the scaled lookup with a gradient by sorted
+tokens and the (tied) head's cross entropy without logits.
+
+Both are plain functions on tensors (``embedding_lookup``, ``linear_cross_entropy``); ``use_libofhip_vocab`` routes a Hugging Face causal LM
+through them.  They stand beside ``towers.use_libofhip_lm_loss``, which computes the same loss from materialised logits, and
+``sparse_rows``, which trains two rows of a frozen table.  GPU tensors only, like everything that runs on libofhip.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..hip import abi
+from ..hip.ops import BF16, F32, Ops
+
+_REDUCTION = {"none": abi.CE_NONE, "mean": abi.CE_MEAN, "sum": abi.CE_SUM}
+
+
+def _rows16(t):
+    """``t`` with unit column stride and rows that begin at multiples of 16 bytes (itself where it has them)."""
+    per = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.stride(0) % per == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    return t.contiguous() if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, table, labels, ignore_index, reduction, logit_scale, piece, ops):
+        x, w = _rows16(hidden), _rows16(table)
+        rows, d = x.shape
+        loss_rows = torch.empty(rows, dtype=F32, device=x.device)
+        loss = torch.empty((), dtype=F32, device=x.device) if reduction != abi.CE_NONE else None
+        state = ops.linear_ce_state(rows, d, x.device)
+        kw = dict(ignore_index=ignore_index, logit_scale=logit_scale, reduction=reduction)
+        ops.linear_ce_fwd(x, w, labels, state, loss_rows, loss, **kw)
+        ctx.save_for_backward(x, w, labels, state)
+        ctx.kw, ctx.ops = dict(kw, piece=piece), ops
+        return loss_rows if loss is None else loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, w, labels, state = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        dx = torch.empty(x.shape, dtype=BF16, device=x.device) if need_x else None
+        dw = torch.empty(w.shape, dtype=BF16, device=w.device) if need_w else None
+        with torch.cuda.device_of(x):
+            ctx.ops.linear_ce_bwd(x, w, labels, state, g.to(F32).contiguous(), dx, dw, **ctx.kw)
+        return dx, dw, None, None, None, None, None, None
+
+
+def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction="mean", logit_scale=1.0, piece=0, ops=None):
+    """Softmax cross entropy of the logits ``logit_scale * hidden @ table.T``, which are never stored:
+    ``F.cross_entropy(logits.float(), labels, ignore_index=..., reduction=...)`` with fp32 statistics of unrounded logits.
+
+    hidden (..., d) and table (vocabulary, d): bfloat16, or any floating type under bf16 autocast (cast as ``F.linear`` casts); d a
+    multiple of 8.  labels (...): int64, already shifted.  reduction "mean" (over the labels that count: NaN without any), "sum" or
+    "none" (one fp32 loss per label, 0 where ignored).  A label outside the vocabulary that is not ``ignore_index`` makes the loss NaN and
+    has no gradient.  Gradients come in bfloat16 for both operands, through fp32 sums; ``piece``: vocabulary rows the backward
+    holds a logits gradient of at a time (0: chosen, 128 MB of it)."""
+    if reduction not in _REDUCTION:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {reduction!r}")
+    if hidden.shape[:-1] != labels.shape:
+        raise ValueError(f"labels {tuple(labels.shape)} do not fit hidden states {tuple(hidden.shape)}")
+    if table.dim() != 2 or table.shape[1] != hidden.shape[-1] or table.shape[0] == 0:
+        raise ValueError(f"table {tuple(table.shape)} does not fit hidden states {tuple(hidden.shape)}")
+    if hidden.shape[-1] % 8:
+        raise ValueError(f"the hidden size must be a multiple of 8, got {hidden.shape[-1]}")
+    if labels.dtype != torch.int64:
+        raise TypeError(f"labels must be int64, got {labels.dtype}")
+    if piece < 0:
+        raise ValueError("piece must not be negative")
+    if len({hidden.device, table.device, labels.device}) != 1:
+        raise ValueError(f"hidden, table and labels are on {hidden.device}, {table.device} and {labels.device}")
+    ops = _ops_for(hidden, ops)
+    dev = hidden.device.type
+    if torch.is_autocast_enabled(dev) and torch.get_autocast_dtype(dev) == BF16:
+        hidden, table = hidden.to(BF16), table.to(BF16)
+    if hidden.dtype != BF16 or table.dtype != BF16:
+        raise TypeError(f"linear_cross_entropy takes bfloat16 operands (or runs under bf16 autocast), got {hidden.dtype} and {table.dtype}")
+    x, y = hidden.reshape(-1, hidden.shape[-1]), labels.reshape(-1).contiguous()
+    if x.shape[0] == 0:          # no rows: torch's values, zero gradients
+        zero = (hidden.sum() + table[:0].sum()).to(F32)
+        return zero.new_zeros(labels.shape) if reduction == "none" else zero / 0.0 if reduction == "mean" else zero
+    with torch.autocast(dev, enabled=False), torch.cuda.device_of(x):
+        out = _LinearCrossEntropy.apply(x, table, y, int(ignore_index), _REDUCTION[reduction], float(logit_scale), int(piece), ops)
+    return out.view(labels.shape) if reduction == "none" else out
+
+
+def _ops_for(t, ops):
+    """the given Ops (tests: the emulator's), else the product's, which takes GPU tensors only"""
+    if ops is not None:
+        return ops
+    if not t.is_cuda:
+        raise RuntimeError("libofhip runs on GPU tensors: there is no CPU fallback")
+    return Ops.default()

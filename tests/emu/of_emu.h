@@ -268,20 +268,31 @@ OF_DEV void of_wait_lgkm0() {}
 OF_DEV void of_wait_vm0_visible() {}
 struct of_buf_t {
     const char* base;
+    unsigned bytes;      // loads at or behind base + bytes return zeros (the hardware's range check)
 };
-OF_DEV of_buf_t of_buf_make(const void* base) { return of_buf_t{(const char*)base}; }
-OF_DEV u32x4 of_buf_load16(of_buf_t b, unsigned voff, unsigned soff) { return *(const u32x4*)(b.base + voff + soff); }
+OF_DEV of_buf_t of_buf_make(const void* base) { return of_buf_t{(const char*)base, 0xffffffffu}; }
+OF_DEV of_buf_t of_buf_make_n(const void* base, unsigned bytes) { return of_buf_t{(const char*)base, bytes}; }
+OF_DEV u32x4 of_buf_load16(of_buf_t b, unsigned voff, unsigned soff) {
+    const unsigned long long at = (unsigned long long)voff + soff;
+    if (at + 16 > b.bytes) {
+        u32x4 v = {0u, 0u, 0u, 0u};
+        for (int e = 0; e < 4; ++e)
+            if (at + 4 * e + 4 <= b.bytes) memcpy((char*)&v + 4 * e, b.base + at + 4 * e, 4);
+        return v;
+    }
+    return *(const u32x4*)(b.base + voff + soff);
+}
 OF_DEV void of_buf_store16(of_buf_t b, unsigned voff, unsigned soff, u32x4 v) { *(u32x4*)(const_cast<char*>(b.base) + voff + soff) = v; }
 OF_DEV void of_buf_store16_sys(of_buf_t b, unsigned voff, unsigned soff, u32x4 v) { of_buf_store16(b, voff, soff, v); }
 OF_DEV u32x4 of_buf_load16_sys(of_buf_t b, unsigned voff, unsigned soff) { return of_buf_load16(b, voff, soff); }
 template <bool TRSAFE = true>
 OF_DEV void of_buf_load16_lds(of_buf_t b, unsigned voff, unsigned soff, void* lds_wave_base) {
-    *(u32x4*)((char*)lds_wave_base + (of_emu::g_blk->cur & 63) * 16) = *(const u32x4*)(b.base + voff + soff);
+    *(u32x4*)((char*)lds_wave_base + (of_emu::g_blk->cur & 63) * 16) = of_buf_load16(b, voff, soff);
 }
 OF_DEV unsigned of_lds_base(const void* smem) { return (unsigned)((const char*)smem - of_emu::g_blk->smem); }
 template <bool TRSAFE = true>
 OF_DEV void of_buf_load16_lds_at(of_buf_t b, unsigned voff, unsigned soff, unsigned lds_addr) {
-    *(u32x4*)(of_emu::g_blk->smem + lds_addr + (of_emu::g_blk->cur & 63) * 16) = *(const u32x4*)(b.base + voff + soff);
+    *(u32x4*)(of_emu::g_blk->smem + lds_addr + (of_emu::g_blk->cur & 63) * 16) = of_buf_load16(b, voff, soff);
 }
 OF_DEV void of_barrier_raw() { of_emu::block_barrier(); }
 OF_DEV float of_shfl(float v, int src) {
