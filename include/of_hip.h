@@ -407,6 +407,43 @@ size_t of_linear_ce_workspace_bytes(const OfLinearCeArgs* args, int backward);
 int of_linear_ce_fwd(const OfLinearCeArgs* args, void* stream);
 int of_linear_ce_bwd(const OfLinearCeArgs* args, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------
+ * Lookup in a vocabulary table and its gradient (ABI v12).  table: vocab x d (row stride ldt), fp32 (f32 = 1) or bf16 (f32 = 0); y, dy,
+ * dw have the table's dtype.  Any d, any strides >= d; rows of whole 16-byte vectors at 16-byte addresses are faster.
+ *   of_embedding_fwd: y[i] = scale * table[ids[i]]; NaN in the rows of ids outside [0, vocab) (nothing is read for them)
+ *   of_embedding_bwd: dw[v] = scale * sum over {i: ids[i] = v} dy[i], summed in fp32 in ascending i, EVERY row written (zeros without a
+ *              token); positions whose id is padding_idx (-1: none is) or outside the table add nothing.  Deterministic: the positions are
+ *              sorted by id, no floating-point atomics.  Workspace: of_embedding_bwd_workspace_bytes, 16-byte aligned. */
+int of_embedding_fwd(const long long* ids, long n, const void* table, int f32, long ldt, int vocab, int d, float scale, void* y, long ldy,
+                     void* stream);
+size_t of_embedding_bwd_workspace_bytes(long n, int vocab, int d);
+int of_embedding_bwd(const long long* ids, long n, const void* dy, int f32, long lddy, int vocab, int d, float scale, long long padding_idx,
+                     void* dw, long lddw, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------
+ * One AdamW step over many tensors (ABI v12): the update of of_adamw_clip with the global norm of all gradients taken inside the call.
+ * tensors: a HOST array of n descriptions, copied into kernel arguments (the call may be captured; a replay uses the same pointers).
+ * bits = 32: m and v are fp32.  bits = 8: m and v hold one e4m3 code per element, m_scale and v_scale one fp32 scale per
+ * OF_ADAMW_BLOCK consecutive elements of the tensor (ceil(n / 256) of them): first moment = code * scale, SQUARE ROOT of the second
+ * moment = code * scale.  All-zero codes and scales are a fresh state.  The first moment is rounded to the nearest code, the root of the
+ * second at random in proportion (a hash of tensor's place in the list, element and step: the same call gives the same bits).
+ *   max_norm <= 0: no clipping.  *sumsq receives the squared norm.  A norm that is not finite leaves p, m, v and scales untouched.
+ *   step: 1-based; with applied_steps (device int) the count of applied updates there is advanced and used instead.
+ * Workspace: of_adamw_multi_workspace_bytes(n), 16-byte aligned.  Tensors must not overlap. */
+#define OF_ADAMW_BLOCK 256
+typedef struct OfAdamwTensor {
+    float* p;
+    const void* g;              /* fp32, or bf16 where g_bf16 */
+    void* m; void* v;
+    float* m_scale; float* v_scale;
+    long n;
+    float lr, weight_decay;
+    int g_bf16;
+} OfAdamwTensor;
+size_t of_adamw_multi_workspace_bytes(int n);
+int of_adamw_multi(const OfAdamwTensor* tensors, int n, int bits, double beta1, double beta2, double eps, double max_norm, int step,
+                   int* applied_steps, float* sumsq, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -390,6 +390,20 @@ OF_DEV float of_rows_sum(float x) {
     of_swap_rows32(a, b);
     return a + b;
 }
+// the lanes of the wave in which the predicate holds
+OF_DEV unsigned long long of_ballot(bool p) { return __builtin_amdgcn_ballot_w64(p); }
+// adds to a counter in LDS (integers: the sum does not depend on the order)
+OF_DEV void of_lds_count(int* p, int v) { atomicAdd(p, v); }
+// e4m3 (OCP: 1 sign, 4 exponent, 3 mantissa bits, largest value 448), four to a register: v_cvt_pk_f32_fp8 / v_cvt_pk_fp8_f32 (round to
+// nearest, ties to even; the caller keeps |x| <= 448)
+OF_DEV f32x4 of_fp8x4_to_f32(unsigned u) {
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, true);
+    return f32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+OF_DEV unsigned of_f32_to_fp8x4(f32x4 v) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+}
 // true if the predicate holds in ANY lane of the wave (the result is wave-uniform: scalar branch)
 OF_DEV bool of_wave_any(bool p) { return __builtin_amdgcn_ballot_w64(p) != 0; }
 // 1-ulp hardware reciprocal (v_rcp_f32) instead of the ~12-instruction IEEE division sequence
@@ -460,7 +474,20 @@ OF_DEV float of_wave_sum(float v) {
     v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xf, 0xf, false));
     return of_rows_sum(v);
 }
+// the same tree with max
+OF_DEV float of_wave_max(float v) {
+    v = of_max(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, false)));
+    v = of_max(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xf, 0xf, false)));
+    v = of_max(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xf, 0xf, false)));
+    v = of_max(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xf, 0xf, false)));
+    return of_rows_max(v);
+}
 #else
+OF_DEV float of_wave_max(float v) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v = of_max(v, of_shfl_xor(v, m));
+    return v;
+}
 OF_DEV float of_wave_sum(float v) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) v += of_shfl_xor(v, m);

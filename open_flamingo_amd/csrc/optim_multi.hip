@@ -1,0 +1,328 @@
+// AdamW over many tensors at once (gfx950, HBM-bound), moments in fp32 or in 8 bits; the clip by the global norm is part of the step.
+//   g' = g min(1, max_norm / (|g| + 1e-6));   m = b1 m + (1 - b1) g';   v = b2 v + (1 - b2) g'^2
+//   p  = p (1 - lr wd) - lr / (1 - b1^t)  m / (sqrt(v / (1 - b2^t)) + eps)
+// An element costs 28 bytes of traffic with fp32 moments and gradients, 16 with 8-bit moments, and 4 more for the norm.  One launch takes
+// up to 48 tensors (their pointers travel in the kernel arguments: nothing to keep in step on the device, safe to capture); a
+// workgroup takes 4096 elements of one tensor.
+//
+// 8-bit moments: e4m3 codes with one fp32 scale (largest magnitude / 448) per 256 consecutive elements of a tensor.
+//   * The first moment is rounded to the nearest code: it moves by a tenth of its distance to g' every step, more than half a code.
+//   * The second moment is held as its square root, which halves the range of exponents a code has to cover.  It moves by a thousandth
+//     (b2 = 0.999) of its distance to g'^2 a step, far less than half a code (1/16 ... 1/32): rounded to the nearest it would stand
+//     still.  It is rounded up or down at random in proportion, so that its expectation is exact; the 20 random bits are a hash of (tensor,
+//     element, step): the same call gives the same bits.  From above zero it never goes to zero (m / (0 + eps) would explode).
+//   * The parameter's own update uses the moments in fp32, before they are rounded.
+#include "of_platform.h"
+#include "../../include/of_hip.h"
+
+namespace {
+
+constexpr int MT_MAX = 48;                  // tensors per launch: 48 x 72 bytes of descriptors in the kernel arguments
+constexpr int MT_CHUNK = 4096;              // elements per workgroup = 16 blocks of 256, four for each wave
+constexpr int MT_PARTS = 1024;              // partial sums of squares per launch of the norm
+constexpr int BLOCK = OF_ADAMW_BLOCK;
+
+struct MtTensor {
+    float* p; const void* g; void* m; void* v; float* ms; float* vs;
+    long n;
+    float lr, wd;
+    int flags;                              // 1: bf16 gradient, 2: all pointers aligned for four elements at a time
+    int ordinal;
+};
+// what the step's launches share, on the device
+struct MtStep {
+    float coef;                             // gradient factor of the clip; negative: a norm that is not finite, the step is left out
+    float inv_sqrt_bc2, inv_bc1;
+    int t;
+};
+struct MtArgs {
+    int n;
+    int chunk_end[MT_MAX];                  // cumulative chunks
+    float beta1, omb1, beta2, omb2, eps;
+    MtStep* step;
+    float* parts;
+    MtTensor t[MT_MAX];
+};
+static_assert(sizeof(MtArgs) <= 4096, "kernel arguments");
+struct MtBeginArgs {
+    const float* parts; long count;
+    float max_norm; double beta1, beta2;
+    int step; int* applied;
+    MtStep* out; float* sumsq;
+};
+
+// the tensor a chunk belongs to (branches are uniform; the table sits in the kernel arguments)
+OF_DEV int mt_find(const MtArgs& a, int chunk, int& first) {
+    int lo = 0, hi = a.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (chunk < a.chunk_end[mid]) hi = mid;
+        else lo = mid + 1;
+    }
+    lo = of_uniform(lo);
+    first = lo ? a.chunk_end[lo - 1] : 0;
+    return lo;
+}
+
+// four elements at i of a float / bf16 array; zeros behind n
+OF_DEV f32x4 mt_load(const void* base, int bf16, bool vec, long i, long n) {
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+    if (vec && i + 4 <= n) {
+        if (!bf16) return *(const f32x4*)((const float*)base + i);
+        const u32x2 u = *(const u32x2*)((const bf16_t*)base + i);
+        return f32x4{of_bf16_to_f32((bf16_t)(u[0] & 0xffff)), of_bf16_to_f32((bf16_t)(u[0] >> 16)), of_bf16_to_f32((bf16_t)(u[1] & 0xffff)),
+                     of_bf16_to_f32((bf16_t)(u[1] >> 16))};
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e < n) r[e] = bf16 ? of_bf16_to_f32(((const bf16_t*)base)[i + e]) : ((const float*)base)[i + e];
+    return r;
+}
+OF_DEV void mt_store(float* base, bool vec, long i, long n, f32x4 x) {
+    if (vec && i + 4 <= n) {
+        *(f32x4*)(base + i) = x;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e < n) base[i + e] = x[e];
+}
+OF_DEV unsigned mt_load_codes(const void* base, bool vec, long i, long n) {
+    if (vec && i + 4 <= n) return *(const unsigned*)((const unsigned char*)base + i);
+    unsigned u = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e < n) u |= (unsigned)((const unsigned char*)base)[i + e] << (8 * e);
+    return u;
+}
+OF_DEV void mt_store_codes(void* base, bool vec, long i, long n, unsigned u) {
+    if (vec && i + 4 <= n) {
+        *(unsigned*)((unsigned char*)base + i) = u;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e < n) ((unsigned char*)base)[i + e] = (unsigned char)(u >> (8 * e));
+}
+
+// ------------------------------------------------------------------------------------------------ the norm
+// workgroup b of MT_PARTS sums the squares of chunks b, b + MT_PARTS, ...: the slot -> element assignment depends on the sizes alone
+OF_GLOBAL void OF_BOUNDS(256, 4) mt_sumsq_kernel(MtArgs a) {
+    float* red = (float*)of_smem();
+    const int tid = of_tid(), all = a.chunk_end[a.n - 1];
+    float s = 0.f;
+    for (int c = of_bid_x(); c < all; c += MT_PARTS) {
+        int first;
+        const MtTensor& t = a.t[mt_find(a, c, first)];
+        const long base = (long)(c - first) * MT_CHUNK + tid * 4;
+        f32x4 g[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) g[u] = mt_load(t.g, t.flags & 1, t.flags & 2, base + u * 1024, t.n);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s += (g[u][0] * g[u][0] + g[u][1] * g[u][1]) + (g[u][2] * g[u][2] + g[u][3] * g[u][3]);
+    }
+    s = of_wave_sum(s);
+    if ((tid & 63) == 0) red[tid >> 6] = s;
+    of_sync();
+    if (tid == 0) a.parts[of_bid_x()] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// one workgroup: the partial sums in a fixed order, then everything a step needs once -- bias corrections in 64 bits (1 - 0.999^t loses
+// four digits in 32 at small t).  `applied` counts the steps that were not left out.
+OF_GLOBAL void OF_BOUNDS(256, 1) mt_begin_kernel(MtBeginArgs a) {
+    float* red = (float*)of_smem();
+    const int tid = of_tid();
+    float s = 0.f;
+    for (long i = tid; i < a.count; i += 256) s += a.parts[i];
+    s = of_wave_sum(s);
+    if ((tid & 63) == 0) red[tid >> 6] = s;
+    of_sync();
+    if (tid == 0) {
+        const float sum = (red[0] + red[1]) + (red[2] + red[3]), norm = sqrtf(sum);
+        const bool finite = norm < 3.0e38f;
+        *a.sumsq = sum;
+        int t = a.step;
+        if (a.applied) {
+            t = *a.applied + 1;
+            if (finite) *a.applied = t;
+        }
+        float coef = a.max_norm > 0.f ? a.max_norm / (norm + 1e-6f) : 1.0f;
+        if (!(coef < 1.0f)) coef = 1.0f;
+        a.out->coef = finite ? coef : -1.0f;
+        a.out->t = t;
+        a.out->inv_bc1 = (float)(1.0 / (1.0 - pow(a.beta1, (double)t)));
+        a.out->inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ the update
+// 20 random bits of (tensor, element, step): multiplications by odd constants and shifts, every input bit reaches every output bit
+OF_DEV unsigned mt_random20(unsigned key, long i) {
+    unsigned x = ((unsigned)i ^ key) * 0x9E3779B1u;
+    x = (x ^ (x >> 15)) * 0x85157AF5u;
+    x = (x ^ (x >> 13)) * 0x9E3779B1u;
+    return (x ^ (x >> 16)) & 0xFFFFFu;
+}
+// q in [0, 448] to a neighbouring e4m3 value, the upper one with the probability of q's place between the two (u: 20 random bits);
+// above zero stays above zero
+OF_DEV float mt_round_random(float q, unsigned u) {
+    if (!(q > 0.f)) return 0.f;
+    float r;
+    if (q >= 0.015625f) {                   // 2^-6, the smallest normal value: 20 of the 23 mantissa bits go
+        r = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, q) + u) & 0xFFF00000u);
+        r = r < 448.0f ? r : 448.0f;
+    } else {                                // below, values are 2^-9 apart
+        r = floorf(q * 512.0f + (float)u * 0x1p-20f) * (1.0f / 512.0f);
+        r = r > (1.0f / 512.0f) ? r : 1.0f / 512.0f;
+    }
+    return r;
+}
+
+struct MtHyper {
+    float coef, step_size, inv_sqrt_bc2, decay, beta1, omb1, beta2, omb2, eps;
+};
+OF_DEV void mt_update(const MtHyper& h, f32x4& p, f32x4 g, f32x4& m, f32x4& v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float ge = h.coef * g[e];
+        m[e] = h.beta1 * m[e] + h.omb1 * ge;
+        v[e] = h.beta2 * v[e] + h.omb2 * ge * ge;
+        p[e] = h.decay * p[e] - h.step_size * (m[e] / (sqrtf(v[e]) * h.inv_sqrt_bc2 + h.eps));
+    }
+}
+
+template <int BITS>
+OF_GLOBAL void OF_BOUNDS(256, 4) mt_adamw_kernel(MtArgs a) {
+    const MtStep st = *a.step;
+    if (st.coef < 0.f) return;
+    int first;
+    const MtTensor& t = a.t[mt_find(a, of_bid_x(), first)];
+    const int tid = of_tid(), lane = tid & 63, wave = tid >> 6, bf16 = t.flags & 1;
+    const bool vec = t.flags & 2;
+    const long n = t.n, base = (long)(of_bid_x() - first) * MT_CHUNK + wave * (4 * BLOCK) + lane * 4;
+    const MtHyper h{st.coef, t.lr * st.inv_bc1, st.inv_sqrt_bc2, 1.0f - t.lr * t.wd, a.beta1, a.omb1, a.beta2, a.omb2, a.eps};
+    f32x4 p[4], g[4], m[4], v[4];
+    unsigned mc[4], vc[4];
+    float ms[4], vs[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const long i = base + u * BLOCK;
+        p[u] = mt_load(t.p, 0, vec, i, n);
+        g[u] = mt_load(t.g, bf16, vec, i, n);
+        if (BITS == 32) {
+            m[u] = mt_load(t.m, 0, vec, i, n);
+            v[u] = mt_load(t.v, 0, vec, i, n);
+        } else {
+            mc[u] = mt_load_codes(t.m, vec, i, n);
+            vc[u] = mt_load_codes(t.v, vec, i, n);
+            const long b = i / BLOCK;           // the wave's block
+            ms[u] = i - lane * 4 < n ? t.ms[b] : 0.f;
+            vs[u] = i - lane * 4 < n ? t.vs[b] : 0.f;
+        }
+    }
+    const unsigned key = (unsigned)st.t * 0x9E3779B1u + (unsigned)t.ordinal * 0x85157AF5u;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const long i = base + u * BLOCK;
+        if (BITS == 32) {
+            mt_update(h, p[u], g[u], m[u], v[u]);
+            mt_store(t.p, vec, i, n, p[u]);
+            mt_store((float*)t.m, vec, i, n, m[u]);
+            mt_store((float*)t.v, vec, i, n, v[u]);
+        } else {
+            m[u] = of_fp8x4_to_f32(mc[u]);
+            v[u] = of_fp8x4_to_f32(vc[u]);
+            float tm = 0.f, tr = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                m[u][e] *= ms[u];
+                v[u][e] *= vs[u];
+                v[u][e] *= v[u][e];
+            }
+            mt_update(h, p[u], g[u], m[u], v[u]);
+            mt_store(t.p, vec, i, n, p[u]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[u][e] = sqrtf(v[u][e]);
+                if (i + e >= n) m[u][e] = v[u][e] = 0.f;
+                tm = of_max(tm, fabsf(m[u][e]));
+                tr = of_max(tr, v[u][e]);
+            }
+            tm = of_wave_max(tm);
+            tr = of_wave_max(tr);
+            const float im = 448.0f / of_max(tm, 1e-30f), ir = 448.0f / of_max(tr, 1e-30f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float q = m[u][e] * im;
+                m[u][e] = q > 448.0f ? 448.0f : q < -448.0f ? -448.0f : q;
+                const float r = v[u][e] * ir;
+                v[u][e] = mt_round_random(r > 448.0f ? 448.0f : r, mt_random20(key, i + e));
+            }
+            mt_store_codes(t.m, vec, i, n, of_f32_to_fp8x4(m[u]));
+            mt_store_codes(t.v, vec, i, n, of_f32_to_fp8x4(v[u]));
+            if (lane == 0 && i < n) {
+                t.ms[i / BLOCK] = tm / 448.0f;
+                t.vs[i / BLOCK] = tr / 448.0f;
+            }
+        }
+    }
+}
+
+int mt_launches(int n) { return (n + MT_MAX - 1) / MT_MAX; }
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+}  // namespace
+
+extern "C" size_t of_adamw_multi_workspace_bytes(int n) { return n > 0 ? up256(sizeof(MtStep)) + (size_t)mt_launches(n) * MT_PARTS * sizeof(float) : 0; }
+
+extern "C" int of_adamw_multi(const OfAdamwTensor* tensors, int n, int bits, double beta1, double beta2, double eps, double max_norm, int step, int* applied_steps,
+                              float* sumsq, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!tensors || n <= 0 || (bits != 8 && bits != 32) || !sumsq || !workspace || (step <= 0 && !applied_steps)) return OF_E_ARG;
+    if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0)) return OF_E_ARG;
+    if (workspace_bytes < of_adamw_multi_workspace_bytes(n)) return OF_E_WORKSPACE;
+    if ((uintptr_t)workspace & 15) return OF_E_ALIGN;
+    for (int i = 0; i < n; ++i) {
+        const OfAdamwTensor& t = tensors[i];
+        if (!t.p || !t.g || !t.m || !t.v || t.n <= 0 || (bits == 8 && (!t.m_scale || !t.v_scale))) return OF_E_ARG;
+        if (((uintptr_t)t.p & 3) || ((uintptr_t)t.g & (t.g_bf16 ? 1 : 3)) || (bits == 32 && (((uintptr_t)t.m & 3) || ((uintptr_t)t.v & 3))) || ((uintptr_t)t.m_scale & 3) || ((uintptr_t)t.v_scale & 3))
+            return OF_E_ALIGN;
+        if (t.n > (long)MT_CHUNK << 24) return OF_E_SHAPE;      // 2^36 elements of one tensor
+    }
+    of_stream_t s = (of_stream_t)stream;
+    MtStep* st = (MtStep*)workspace;
+    float* parts = (float*)((char*)workspace + up256(sizeof(MtStep)));
+    const int launches = mt_launches(n);
+    auto pack = [&](int l, MtArgs& a) {
+        a = MtArgs{};
+        long end = 0;
+        for (int i = l * MT_MAX; i < n && i < (l + 1) * MT_MAX; ++i) {
+            const OfAdamwTensor& t = tensors[i];
+            MtTensor& d = a.t[a.n];
+            d.p = t.p; d.g = t.g; d.m = t.m; d.v = t.v; d.ms = t.m_scale; d.vs = t.v_scale; d.n = t.n; d.lr = t.lr; d.wd = t.weight_decay;
+            const uintptr_t wide = (uintptr_t)t.p | (t.g_bf16 ? (uintptr_t)t.g << 1 : (uintptr_t)t.g);
+            const uintptr_t state = (uintptr_t)t.m | (uintptr_t)t.v;
+            d.flags = (t.g_bf16 ? 1 : 0) | (!(wide & 15) && !(state & (bits == 32 ? 15 : 3)) ? 2 : 0);
+            d.ordinal = i;
+            end += (t.n + MT_CHUNK - 1) / MT_CHUNK;
+            a.chunk_end[a.n++] = (int)end;
+        }
+        a.beta1 = (float)beta1; a.omb1 = (float)(1.0 - beta1); a.beta2 = (float)beta2; a.omb2 = (float)(1.0 - beta2); a.eps = (float)eps;
+        a.step = st;
+        a.parts = parts + (size_t)l * MT_PARTS;
+        return end;
+    };
+    MtArgs a;
+    for (int l = 0; l < launches; ++l)
+        if (pack(l, a) >= 1l << 31) return OF_E_SHAPE;
+    for (int l = 0; l < launches; ++l) {
+        pack(l, a);
+        const int rc = of_launch(mt_sumsq_kernel, of_dim3{MT_PARTS, 1, 1}, 256, 4 * sizeof(float), s, a);
+        if (rc) return rc;
+    }
+    const MtBeginArgs b{parts, (long)launches * MT_PARTS, (float)max_norm, beta1, beta2, step, applied_steps, st, sumsq};
+    int rc = of_launch(mt_begin_kernel, of_dim3{1, 1, 1}, 256, 4 * sizeof(float), s, b);
+    for (int l = 0; l < launches && !rc; ++l) {
+        const unsigned grid = (unsigned)pack(l, a);
+        rc = bits == 8 ? of_launch(mt_adamw_kernel<8>, of_dim3{grid, 1, 1}, 256, 0, s, a) : of_launch(mt_adamw_kernel<32>, of_dim3{grid, 1, 1}, 256, 0, s, a);
+    }
+    return rc;
+}

@@ -101,6 +101,14 @@ class OfLinearCeArgs(C.Structure):
     ]
 
 
+ADAMW_BLOCK = 256
+
+
+class OfAdamwTensor(C.Structure):
+    _fields_ = [("p", vp), ("g", vp), ("m", vp), ("v", vp), ("m_scale", vp), ("v_scale", vp), ("n", C.c_long), ("lr", C.c_float),
+                ("weight_decay", C.c_float), ("g_bf16", C.c_int)]
+
+
 PROTOTYPES = {
     "of_abi_version": (C.c_int, []),
     "of_build_kind": (C.c_int, []),
@@ -152,6 +160,12 @@ PROTOTYPES = {
     "of_linear_ce_workspace_bytes": (C.c_size_t, [C.POINTER(OfLinearCeArgs), C.c_int]),
     "of_linear_ce_fwd": (C.c_int, [C.POINTER(OfLinearCeArgs), vp]),
     "of_linear_ce_bwd": (C.c_int, [C.POINTER(OfLinearCeArgs), vp]),
+    "of_embedding_fwd": (C.c_int, [vp, C.c_long, vp, C.c_int, C.c_long, C.c_int, C.c_int, C.c_float, vp, C.c_long, vp]),
+    "of_embedding_bwd_workspace_bytes": (C.c_size_t, [C.c_long, C.c_int, C.c_int]),
+    "of_embedding_bwd": (C.c_int, [vp, C.c_long, vp, C.c_int, C.c_long, C.c_int, C.c_int, C.c_float, C.c_longlong, vp, C.c_long, vp, C.c_size_t, vp]),
+    "of_adamw_multi_workspace_bytes": (C.c_size_t, [C.c_int]),
+    "of_adamw_multi": (C.c_int, [C.c_char_p, C.c_int, C.c_int, C.c_double, C.c_double, C.c_double, C.c_double, C.c_int, vp, vp, vp,
+                                 C.c_size_t, vp]),
     "of_reduce_rows_strided": (C.c_int, [vp, C.c_int, C.c_long, C.c_int, C.c_long, C.c_int, vp, vp]),
 }
 

@@ -5,6 +5,7 @@ handle and a way to obtain the current stream.  The product instance (``Ops.defa
 ``libofhip.so`` + the current HIP stream and is the only one ``open_flamingo_amd.src`` ever uses.
 """
 import ctypes as C
+import struct
 
 import torch
 
@@ -498,6 +499,34 @@ class Ops:
                 setattr(a, "ld" + name, max(t.stride(0), a.d))
         ws = self._linear_ce_workspace(a, 1, x.device)          # noqa: F841
         self._chk(self.lib.of_linear_ce_bwd(C.byref(a), self._stream()), "of_linear_ce_bwd")
+
+    # ------------------------------------------------------------------ lookup in a vocabulary table
+    def embedding_fwd(self, ids, table, out, scale=1.0):
+        """out[i] = scale * table[ids[i]] (fp32 or bf16 like the table); NaN rows for ids outside it."""
+        assert ids.dtype == torch.int64 and ids.dim() == 1 and ids.is_contiguous() and out.dtype == table.dtype
+        assert out.shape == (ids.numel(), table.shape[1]) and table.stride(1) == 1 and out.stride(1) == 1
+        d = table.shape[1]
+        self._chk(self.lib.of_embedding_fwd(ids.data_ptr(), ids.numel(), table.data_ptr(), _is_f32(table), max(table.stride(0), d), table.shape[0], d,
+                                            scale, out.data_ptr(), max(out.stride(0), d), self._stream()), "of_embedding_fwd")
+
+    def embedding_bwd(self, ids, dy, dw, scale=1.0, padding_idx=-1):
+        """dw[v] = scale * sum of dy[i] over ids[i] == v, every row written; positions with padding_idx or an id outside dw add nothing."""
+        assert ids.dtype == torch.int64 and ids.dim() == 1 and ids.is_contiguous() and dy.dtype == dw.dtype
+        assert dy.shape == (ids.numel(), dw.shape[1]) and dy.stride(1) == 1 and dw.stride(1) == 1
+        n, (vocab, d) = ids.numel(), dw.shape
+        ws = torch.empty(self.lib.of_embedding_bwd_workspace_bytes(n, vocab, d), dtype=torch.uint8, device=dw.device)
+        self._chk(self.lib.of_embedding_bwd(ids.data_ptr(), n, dy.data_ptr(), _is_f32(dy), max(dy.stride(0), d), vocab, d, scale, padding_idx,
+                                            dw.data_ptr(), max(dw.stride(0), d), ws.data_ptr(), ws.numel(), self._stream()), "of_embedding_bwd")
+
+    # ------------------------------------------------------------------ AdamW over many tensors
+    def adamw_multi(self, tensors, sumsq, *, bits, betas=(0.9, 0.999), eps=1e-8, max_norm=0.0, step=0, applied=None):
+        """One clip + AdamW step (of_adamw_multi).  tensors: the fields of OfAdamwTensor, one tensor's behind the other's, checked by the
+        caller (train/optim.py::adamw_step)."""
+        n = len(tensors) // 10
+        table = struct.pack("=" + "7q2fi4x" * n, *tensors)
+        ws = torch.empty(self.lib.of_adamw_multi_workspace_bytes(n), dtype=torch.uint8, device=sumsq.device)
+        self._chk(self.lib.of_adamw_multi(table, n, bits, betas[0], betas[1], eps, max_norm, step, _p(applied), sumsq.data_ptr(),
+                                          ws.data_ptr(), ws.numel(), self._stream()), "of_adamw_multi")
 
     def quick_gelu(self, x, out=None):
         assert x.dtype == BF16 and x.is_contiguous()

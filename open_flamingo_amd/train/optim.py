@@ -15,6 +15,7 @@ cross-attention parameters (open_flamingo/train/train.py:392-408).  Differences,
 """
 import torch
 
+from ..hip import abi
 from ..hip.ops import BF16, F32, Ops
 
 
@@ -396,3 +397,67 @@ class FlatAdamW(torch.optim.Optimizer):
         """Global gradient norm of the last step() (device scalar tensor, pre-clip)."""
         gs = 1.0 / self.reducer.world if getattr(self.reducer, "holds_sum", False) else 1.0
         return self._sumsq.sqrt() * gs
+
+
+# ---------------------------------------------------------------------------------------- AdamW over any list of tensors
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=0, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_norm=0.0,
+               exp_avg_scales=None, exp_avg_sq_scales=None, applied=None, ops=None):
+    """One AdamW update of ``params`` in place, all tensors in a few launches, with the clip by the norm of all gradients in the same call.
+
+    params: fp32; grads: fp32 or bf16 (left as they are); exp_avgs, exp_avg_sqs: fp32, or -- with ``exp_avg_scales`` and
+    ``exp_avg_sq_scales`` -- 8-bit codes (torch.float8_e4m3fn) of the first moment and of the SQUARE ROOT of the second, one fp32 scale
+    per 256 consecutive elements (value = code * scale; zeros are a fresh state; ``adamw_state`` makes them).  All contiguous, on one
+    device, none overlapping another.  lr, weight_decay: one value, or one per tensor.  max_norm <= 0: no clipping.
+
+    step: 1-based count of this update; ``applied``, a device int32 counter, replaces it, and counts the updates that were applied.  A
+    gradient norm that is not finite leaves everything untouched (no host synchronisation).  Returns the squared norm (1, fp32)."""
+    n = len(params)
+    coded = exp_avg_scales is not None or exp_avg_sq_scales is not None
+    lists = [grads, exp_avgs, exp_avg_sqs] + ([exp_avg_scales or (), exp_avg_sq_scales or ()] if coded else [])
+    if n == 0 or any(len(ts) != n for ts in lists):
+        raise ValueError(f"{n} parameters with {[len(ts) for ts in lists]} gradients and states")
+    if applied is None and step < 1:
+        raise ValueError(f"step counts from 1, got {step}")
+    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0):
+        raise ValueError(f"betas {betas}, eps {eps}")
+    lrs, wds = (list(x) if isinstance(x, (list, tuple)) else [x] * n for x in (lr, weight_decay))
+    if len(lrs) != n or len(wds) != n:
+        raise ValueError(f"{len(lrs)} learning rates and {len(wds)} weight decays for {n} parameters")
+    # one pass over the tensors: checks and descriptions (host time of a call, ~2 us a tensor)
+    dev, state, block = params[0].get_device(), torch.float8_e4m3fn if coded else F32, abi.ADAMW_BLOCK
+    table, at = [], set()
+    for i in range(n):
+        p, g, m, v = params[i], grads[i], exp_avgs[i], exp_avg_sqs[i]
+        k, pp = p.numel(), p.data_ptr()
+        bf16 = g.dtype is BF16
+        if not (p.dtype is F32 and (bf16 or g.dtype is F32) and m.dtype is state and v.dtype is state and g.numel() == k and m.numel() == k and v.numel() == k
+                and p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()
+                and p.get_device() == dev and g.get_device() == dev and m.get_device() == dev and v.get_device() == dev):
+            raise ValueError(f"tensor {i}: parameter, gradient and states must be contiguous, of one size, on one device, fp32 (gradient: or bf16; states: {state}), got "
+                             + ", ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in (p, g, m, v)))
+        a = b = 0
+        if coded:
+            ms, vs = exp_avg_scales[i], exp_avg_sq_scales[i]
+            if not (ms.dtype is F32 and vs.dtype is F32 and ms.is_contiguous() and vs.is_contiguous() and ms.numel() == vs.numel() == -(-k // block)
+                    and ms.get_device() == dev and vs.get_device() == dev):
+                raise ValueError(f"tensor {i}: one fp32 scale per {block} elements ({-(-k // block)} here), got {ms.dtype} {ms.numel()} and {vs.dtype} {vs.numel()}")
+            a, b = ms.data_ptr(), vs.data_ptr()
+        if k:
+            if pp in at:
+                raise ValueError(f"parameter {i} is listed twice")
+            at.add(pp)
+            table += (pp, g.data_ptr(), m.data_ptr(), v.data_ptr(), a, b, k, lrs[i], wds[i], bf16)
+    device = params[0].device
+    if applied is not None and (applied.dtype != torch.int32 or applied.numel() != 1 or applied.device != device):
+        raise ValueError("applied: one int32 on the parameters' device")
+    if ops is None:
+        if dev < 0:
+            raise RuntimeError("libofhip runs on GPU tensors: there is no CPU fallback")
+        ops = Ops.default()
+    with torch.no_grad(), torch.cuda.device_of(params[0]):
+        sumsq = torch.empty(1, dtype=F32, device=device)
+        if not table:
+            return sumsq.zero_()
+        ops.adamw_multi(table, sumsq, bits=8 if coded else 32, betas=betas, eps=eps, max_norm=max_norm, step=step, applied=applied)
+    torch.autograd.graph.increment_version([*params, *exp_avgs, *exp_avg_sqs, *(exp_avg_scales or ()), *(exp_avg_sq_scales or ())])          # written behind autograd's back
+    return sumsq

@@ -86,6 +86,54 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
     return out.view(labels.shape) if reduction == "none" else out
 
 
+class _EmbeddingLookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, padding_idx, ops):
+        out = torch.empty(ids.numel(), table.shape[1], dtype=table.dtype, device=table.device)
+        ops.embedding_fwd(ids, table, out, scale)
+        ctx.save_for_backward(ids)
+        ctx.shape, ctx.scale, ctx.padding_idx, ctx.ops = table.shape, scale, padding_idx, ops
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (ids,) = ctx.saved_tensors
+        if g.stride(-1) != 1:
+            g = g.contiguous()
+        dw = torch.empty(ctx.shape, dtype=g.dtype, device=g.device)
+        with torch.cuda.device_of(g):
+            ctx.ops.embedding_bwd(ids, g, dw, ctx.scale, ctx.padding_idx)
+        return None, dw, None, None, None
+
+
+def embedding_lookup(ids, table, *, scale=1.0, padding_idx=None, ops=None):
+    """``scale * F.embedding(ids, table, padding_idx)`` for an fp32 or bf16 table, with a dense gradient that is summed in fp32 in a
+    fixed order (the same bits on every run) and rounded once.
+
+    ids: int64 of any shape; an id outside the table gives a row of NaN and no gradient.  padding_idx (None: none; negative: counted
+    from the table's end): that row gets no gradient."""
+    if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
+        raise ValueError(f"table must be (vocabulary, d), got {tuple(table.shape)}")
+    if ids.dtype != torch.int64:
+        raise TypeError(f"ids must be int64, got {ids.dtype}")
+    if table.dtype not in (F32, BF16):
+        raise TypeError(f"the table must be float32 or bfloat16, got {table.dtype}")
+    if ids.device != table.device:
+        raise ValueError(f"ids and table are on {ids.device} and {table.device}")
+    if padding_idx is not None:
+        if not -table.shape[0] <= padding_idx < table.shape[0]:
+            raise ValueError(f"padding_idx {padding_idx} is outside a table of {table.shape[0]} rows")
+        padding_idx %= table.shape[0]
+    ops = _ops_for(table, ops)
+    if ids.numel() == 0:
+        return table[:0].reshape(*ids.shape, table.shape[1]) * scale
+    t = table if table.stride(1) == 1 and table.stride(0) >= table.shape[1] else table.contiguous()
+    with torch.cuda.device_of(t):
+        out = _EmbeddingLookup.apply(ids.reshape(-1).contiguous(), t, float(scale), -1 if padding_idx is None else padding_idx, ops)
+    return out.view(*ids.shape, table.shape[1])
+
+
 def _ops_for(t, ops):
     """the given Ops (tests: the emulator's), else the product's, which takes GPU tensors only"""
     if ops is not None:

@@ -318,6 +318,40 @@ OF_DEV bool of_wave_any(bool p) {
     for (int m = 32; m >= 1; m >>= 1) v |= of_shfl_xor_i(v, m);
     return v != 0;
 }
+OF_DEV unsigned long long of_ballot(bool p) {
+    of_emu::Block* blk = of_emu::g_blk;
+    const int t = blk->cur, w0 = t & ~63;
+    blk->xchg[t][0] = p ? 1 : 0;
+    of_emu::wave_barrier();
+    unsigned long long r = 0;
+    for (int l = 0; l < 64; ++l) r |= (unsigned long long)(blk->xchg[w0 + l][0] != 0) << l;
+    of_emu::wave_barrier();
+    return r;
+}
+OF_DEV void of_lds_count(int* p, int v) { *p += v; }          // the fibers of a workgroup share one thread
+OF_DEV float of_emu_fp8(unsigned b) {
+    const int e = (b >> 3) & 15, m = b & 7;
+    const float v = e == 15 && m == 7 ? NAN : e ? ldexpf(1.f + m / 8.f, e - 7) : ldexpf((float)m, -9);
+    return b & 0x80 ? -v : v;
+}
+OF_DEV unsigned of_emu_to_fp8(float f) {      // round to nearest, ties to even; |f| <= 464
+    const unsigned s = signbit(f) ? 0x80u : 0u;
+    const float a = fabsf(f);
+    if (!(a <= 464.f)) return s | 0x7fu;
+    int e;
+    frexpf(a, &e);
+    const float step = ldexpf(1.f, (e - 1 < -6 ? -6 : e - 1) - 3);
+    const float q = nearbyintf(a / step) * step;
+    for (unsigned c = 0; c < 127; ++c)
+        if (of_emu_fp8(c) == q) return s | c;
+    return s | 0x7eu;
+}
+OF_DEV f32x4 of_fp8x4_to_f32(unsigned u) {
+    return f32x4{of_emu_fp8(u & 255), of_emu_fp8((u >> 8) & 255), of_emu_fp8((u >> 16) & 255), of_emu_fp8(u >> 24)};
+}
+OF_DEV unsigned of_f32_to_fp8x4(f32x4 v) {
+    return of_emu_to_fp8(v[0]) | (of_emu_to_fp8(v[1]) << 8) | (of_emu_to_fp8(v[2]) << 16) | (of_emu_to_fp8(v[3]) << 24);
+}
 OF_DEV void of_pair_rows16(unsigned& a, unsigned& b) {
     const unsigned pa = (unsigned)of_shfl_xor_i((int)a, 16), pb = (unsigned)of_shfl_xor_i((int)b, 16);
     if (((of_emu::g_blk->cur >> 4) & 1) == 0) b = pa;
