@@ -17,6 +17,7 @@ import torch
 
 from ..hip import abi
 from ..hip.ops import BF16, F32, Ops
+from ..src.helpers import _require_hip
 
 
 class FlatAdamW(torch.optim.Optimizer):
@@ -451,8 +452,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=0, lr=1e-3, betas=(
     if applied is not None and (applied.dtype != torch.int32 or applied.numel() != 1 or applied.device != device):
         raise ValueError("applied: one int32 on the parameters' device")
     if ops is None:
-        if dev < 0:
-            raise RuntimeError("libofhip runs on GPU tensors: there is no CPU fallback")
+        _require_hip(params[0], "adamw_step")
         ops = Ops.default()
     with torch.no_grad(), torch.cuda.device_of(params[0]):
         sumsq = torch.empty(1, dtype=F32, device=device)
@@ -461,3 +461,105 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=0, lr=1e-3, betas=(
         ops.adamw_multi(table, sumsq, bits=8 if coded else 32, betas=betas, eps=eps, max_norm=max_norm, step=step, applied=applied)
     torch.autograd.graph.increment_version([*params, *exp_avgs, *exp_avg_sqs, *(exp_avg_scales or ()), *(exp_avg_sq_scales or ())])          # written behind autograd's back
     return sumsq
+
+
+class MultiTensorAdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` for fp32 parameters through ``adamw_step``: every ``step()`` is one call over all parameters that have a gradient,
+    whatever they are (a fully trained vocabulary table included, which ``FlatAdamW`` refuses), with ``clip_grad_norm_(max_norm)`` in it and no
+    host synchronisation; a gradient norm that is not finite skips the step.
+
+    state_bits = 8 holds the moments in 2 bytes an element instead of 8 (see ``adamw_step``).  Groups have their own ``lr`` and
+    ``weight_decay``; betas and eps are common to all (a group of its own values raises).  One count of applied updates serves all parameters
+    (torch keeps one each: the same unless a parameter goes without a gradient for some steps).  ``state_dict`` has torch.optim.AdamW's layout
+    for 32 bits; for 8 bits ``exp_avg`` and ``exp_avg_sq`` hold codes beside ``exp_avg_scale`` and ``exp_avg_sq_scale``."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_norm=0.0, state_bits=32, ops=None):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        self.max_norm, self.state_bits, self.ops = max_norm, state_bits, ops
+        self._applied, self._sumsq = None, None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        for g in self.param_groups:
+            for p in g["params"]:
+                if p.dtype != F32 or not p.is_contiguous():
+                    raise ValueError(f"MultiTensorAdamW takes contiguous fp32 parameters, got {p.dtype} {tuple(p.shape)}")
+
+    def _state_of(self, p):
+        st = self.state[p]
+        if not st:
+            if self.state_bits == 32:
+                st["exp_avg"], st["exp_avg_sq"] = torch.zeros_like(p), torch.zeros_like(p)
+            else:
+                blocks = -(-p.numel() // abi.ADAMW_BLOCK)
+                for k in ("exp_avg", "exp_avg_sq"):
+                    st[k] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
+                    st[k + "_scale"] = torch.zeros(blocks, dtype=F32, device=p.device)
+        return st
+
+    def _counter(self, device):
+        if self._applied is None:
+            self._applied = torch.zeros(1, dtype=torch.int32, device=device)
+        return self._applied
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        first = self.param_groups[0]
+        if any(g["betas"] != first["betas"] or g["eps"] != first["eps"] for g in self.param_groups):
+            raise ValueError("MultiTensorAdamW: betas and eps are common to all parameter groups")
+        params, lrs, wds = [], [], []
+        for g in self.param_groups:
+            for p in g["params"]:
+                if p.grad is not None:
+                    params.append(p)
+                    lrs.append(float(g["lr"]))
+                    wds.append(float(g["weight_decay"]))
+        if not params:
+            return loss
+        states = [self._state_of(p) for p in params]
+        col = lambda k: [st[k] for st in states]          # noqa: E731
+        coded = self.state_bits == 8
+        grads = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in params]
+        self._sumsq = adamw_step(params, grads, col("exp_avg"), col("exp_avg_sq"), lr=lrs, betas=first["betas"], eps=first["eps"], weight_decay=wds,
+                                 max_norm=self.max_norm, exp_avg_scales=col("exp_avg_scale") if coded else None,
+                                 exp_avg_sq_scales=col("exp_avg_sq_scale") if coded else None, applied=self._counter(params[0].device), ops=self.ops)
+        return loss
+
+    def applied_steps(self):
+        """Updates applied so far (host int; synchronises)."""
+        return 0 if self._applied is None else int(self._applied.item())
+
+    def grad_norm(self):
+        """Gradient norm of the last step(), in front of the clip (device scalar)."""
+        return self._sumsq.sqrt()
+
+    def state_dict(self):
+        sd = super().state_dict()
+        step = torch.tensor(float(self.applied_steps()))
+        sd["state"] = {i: dict(step=step.clone(), **st) for i, st in sd["state"].items()}
+        return sd
+
+    def load_state_dict(self, sd):
+        params = [p for g in self.param_groups for p in g["params"]]
+        ids = [i for g in sd["param_groups"] for i in g["params"]]
+        if len(ids) != len(params):
+            raise ValueError(f"optimizer state of {len(ids)} parameters for {len(params)}")
+        new, steps = {}, set()
+        want = F32 if self.state_bits == 32 else torch.float8_e4m3fn
+        for i, p in zip(ids, params):
+            st = sd["state"].get(i)
+            if not st:
+                continue
+            if st["exp_avg"].dtype != want or st["exp_avg"].shape != p.shape or ("exp_avg_scale" in st) != (self.state_bits == 8):
+                raise ValueError(f"the saved state of parameter {i} ({st['exp_avg'].dtype}, {tuple(st['exp_avg'].shape)}) is no {self.state_bits}-bit state of a parameter of shape {tuple(p.shape)}")
+            steps.add(int(float(st["step"])))
+            new[p] = {k: v.detach().clone().to(p.device) for k, v in st.items() if k != "step" and isinstance(v, torch.Tensor)}
+        if len(steps) > 1:
+            raise ValueError(f"parameters at different step counts {sorted(steps)}: one count serves all here")
+        super().load_state_dict({**sd, "state": {}})
+        self.state.update(new)
+        if params:
+            self._counter(params[0].device).fill_(steps.pop() if steps else 0)

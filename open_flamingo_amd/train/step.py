@@ -11,12 +11,15 @@ import torch
 from . import synthetic
 
 
-def build_optimizer(model, lr=1e-4, weight_decay=0.1, reducer=None):
+def build_optimizer(model, lr=1e-4, weight_decay=0.1, reducer=None, multi_tensor=False, state_bits=32):
     """train.py:384-408: wd only on params whose name contains 'gated_cross_attn'.  With a GradReducer on a GPU the
     fused device-side step epilogue (train/optim.py: clip + AdamW over the reducer's flat buckets) is returned; it
-    implements the same update."""
+    implements the same update.  multi_tensor: train/optim.py::MultiTensorAdamW instead (any set of fp32 parameters, a fully trained
+    embedding table included; moments in state_bits = 32 or 8 bits)."""
+    if state_bits != 32 and not multi_tensor:
+        raise ValueError("8-bit optimizer states need multi_tensor=True")
     dense_table = reducer is not None and reducer.embedding is not None and reducer.embedding_rows is None
-    if reducer is not None and reducer.buckets and reducer.buckets[0]["flat"].is_cuda and not dense_table:
+    if not multi_tensor and reducer is not None and reducer.buckets and reducer.buckets[0]["flat"].is_cuda and not dense_table:
         from .optim import FlatAdamW
         return FlatAdamW(reducer, lr=lr, weight_decay=weight_decay)
     if getattr(model, "_of_sparse_rows", None) is not None:
@@ -28,6 +31,9 @@ def build_optimizer(model, lr=1e-4, weight_decay=0.1, reducer=None):
             continue
         (with_wd if "gated_cross_attn" in n else without_wd).append(p)
     groups = [{"params": with_wd, "weight_decay": weight_decay}, {"params": without_wd, "weight_decay": 0.0}]
+    if multi_tensor:
+        from .optim import MultiTensorAdamW
+        return MultiTensorAdamW([g for g in groups if g["params"]], lr=lr, state_bits=state_bits)
     fused = all(p.is_cuda for p in with_wd + without_wd)
     return torch.optim.AdamW(groups, lr=lr, fused=fused)
 
@@ -88,7 +94,8 @@ def train_step(model, reducer, optimizer, batch_mmc4, info, batch_laion=None, lo
     fused = hasattr(optimizer, "reducer")         # FlatAdamW: clip + AdamW + zero_grad in two device passes
     from ..hip import path as _path
     _path.scope_of(getattr(model, "module", model)).twins.clear()         # a gradient twin nobody took in the previous backward (the embedding's) is not kept alive
-    params = None if fused else [p for g in optimizer.param_groups for p in g["params"]]
+    clips = fused or hasattr(optimizer, "max_norm")          # MultiTensorAdamW: clip and skip-on-NaN are part of its step
+    params = None if clips else [p for g in optimizer.param_groups for p in g["params"]]
     if batch_laion is not None:
         with reducer.no_sync() if reducer is not None else contextlib.nullcontext():
             loss_l = forward_loss(model, batch_laion, info, amp, kind="laion")
@@ -101,7 +108,7 @@ def train_step(model, reducer, optimizer, batch_mmc4, info, batch_laion=None, lo
         inner.schedule_vision_prefetch(next_vision_x, amp_dtype=torch.bfloat16 if amp else None)
     loss = forward_loss(model, batch_mmc4, info, amp)
     if nan_check == "device":
-        assert fused, "nan_check='device' relies on the fused step epilogue (FlatAdamW)"
+        assert clips, "nan_check='device' relies on an optimizer that skips a non-finite norm on the device (FlatAdamW, MultiTensorAdamW)"
     elif nan_check and torch.isnan(loss):          # train_utils.py:161-169 (host sync, as in the reference)
         if reducer is not None:
             reducer.zero_grad()
@@ -120,7 +127,7 @@ def train_step(model, reducer, optimizer, batch_mmc4, info, batch_laion=None, lo
     if reducer is not None:
         # waits for the overlapped RCCL all-reduces, restores the two embedding rows; the fused epilogue averages itself
         reducer.finish(average=not hasattr(optimizer, "reducer"))
-    if fused:
+    if clips:
         optimizer.max_norm = clip_norm
         optimizer.step()
     else:

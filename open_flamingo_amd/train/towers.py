@@ -445,6 +445,9 @@ def build_flamingo(family: str = "OF-3B", device="cuda", seed: int = 0, gates: f
         use_libofhip_quick_gelu(model.vision_encoder)
     if lm_loss == "libofhip":
         use_libofhip_lm_loss(model.lang_encoder)
+    if lm_loss == "libofhip_vocab":        # lookup and loss on the vocabulary table, no logits (train/vocab.py)
+        from .vocab import use_libofhip_vocab
+        use_libofhip_vocab(model.lang_encoder)
     if fused_vision:                       # the CLIP tower's encoder as one fused forward (train/frozen_blocks.py)
         model.vision_encoder.fused = fused_vision
     if fused_lm_blocks:                    # whole frozen MPT blocks as one autograd node each (train/frozen_blocks.py)

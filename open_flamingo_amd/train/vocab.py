@@ -5,11 +5,15 @@ Both are plain functions on tensors (``embedding_lookup``, ``linear_cross_entrop
 through them.  They stand beside ``towers.use_libofhip_lm_loss``, which computes the same loss from materialised logits, and
 ``sparse_rows``, which trains two rows of a frozen table.  GPU tensors only, like everything that runs on libofhip.
 """
+import types
+
 import torch
 from torch.autograd.function import once_differentiable
 
 from ..hip import abi
 from ..hip.ops import BF16, F32, Ops
+from ..src import helpers
+from ..src.utils import extend_instance
 
 _REDUCTION = {"none": abi.CE_NONE, "mean": abi.CE_MEAN, "sum": abi.CE_SUM}
 
@@ -71,7 +75,7 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
         raise ValueError("piece must not be negative")
     if len({hidden.device, table.device, labels.device}) != 1:
         raise ValueError(f"hidden, table and labels are on {hidden.device}, {table.device} and {labels.device}")
-    ops = _ops_for(hidden, ops)
+    ops = _ops_for(hidden, ops, "linear_cross_entropy")
     dev = hidden.device.type
     if torch.is_autocast_enabled(dev) and torch.get_autocast_dtype(dev) == BF16:
         hidden, table = hidden.to(BF16), table.to(BF16)
@@ -125,7 +129,7 @@ def embedding_lookup(ids, table, *, scale=1.0, padding_idx=None, ops=None):
         if not -table.shape[0] <= padding_idx < table.shape[0]:
             raise ValueError(f"padding_idx {padding_idx} is outside a table of {table.shape[0]} rows")
         padding_idx %= table.shape[0]
-    ops = _ops_for(table, ops)
+    ops = _ops_for(table, ops, "embedding_lookup")
     if ids.numel() == 0:
         return table[:0].reshape(*ids.shape, table.shape[1]) * scale
     t = table if table.stride(1) == 1 and table.stride(0) >= table.shape[1] else table.contiguous()
@@ -134,10 +138,75 @@ def embedding_lookup(ids, table, *, scale=1.0, padding_idx=None, ops=None):
     return out.view(*ids.shape, table.shape[1])
 
 
-def _ops_for(t, ops):
+def _ops_for(t, ops, what):
     """the given Ops (tests: the emulator's), else the product's, which takes GPU tensors only"""
     if ops is not None:
         return ops
-    if not t.is_cuda:
-        raise RuntimeError("libofhip runs on GPU tensors: there is no CPU fallback")
+    helpers._require_hip(t, what)
     return Ops.default()
+
+
+# ---------------------------------------------------------------------------------------------------------------- Hugging Face LMs
+def _runs_here(t):
+    try:
+        helpers._require_hip(t, "vocabulary table")
+    except (RuntimeError, TypeError):
+        return False
+    return True
+
+
+def _embedding_forward(self, ids):
+    if ids.dtype == torch.int64 and _runs_here(self.weight):
+        return embedding_lookup(ids, self.weight, padding_idx=self.padding_idx)
+    return self._of_eager_forward(ids)
+
+
+class _VocabLossMixin:
+    """``forward(labels=...)`` of a Hugging Face causal LM without logits: the output's ``loss`` comes from ``linear_cross_entropy`` on the
+    last hidden states and the head's weight, its ``logits`` is None.  Without labels nothing changes.  What the operator does not
+    cover (a head with a bias, ``logits_to_keep``, other loss arguments, operands that are not bf16 or under bf16 autocast, the two-row mode of
+    train/sparse_rows.py, whose tap sits behind the logits) takes the LM's own path."""
+
+    def _of_takes(self, labels, kwargs):
+        head = self.get_output_embeddings()
+        w = getattr(head, "weight", None)
+        if labels is None or w is None or getattr(head, "bias", None) is not None or kwargs.get("logits_to_keep") or not _runs_here(w):
+            return False
+        if any(kwargs.get(k) is not None for k in ("num_items_in_batch", "shift_labels", "ignore_index")) or getattr(w, "_of_trained_rows", None) is not None:
+            return False
+        dev = w.device.type
+        amp = torch.is_autocast_enabled(dev) and torch.get_autocast_dtype(dev) == BF16
+        return amp or w.dtype == BF16
+
+    def forward(self, input_ids=None, attention_mask=None, labels=None, **kwargs):
+        if not self._of_takes(labels, kwargs):
+            return super().forward(input_ids=input_ids, attention_mask=attention_mask, labels=labels, **kwargs)
+        seen = []
+        hook = self.base_model.register_forward_hook(lambda mod, args, out: seen.append(out[0]))
+        try:          # the LM's own forward with no position for the head: hidden states, cache and all the rest as it makes them
+            none = torch.empty(0, dtype=torch.int64, device=labels.device)
+            out = super().forward(input_ids=input_ids, attention_mask=attention_mask, logits_to_keep=none, **kwargs)
+        finally:
+            hook.remove()
+        w = self.get_output_embeddings().weight
+        ahead = torch.nn.functional.pad(labels.to(seen[-1].device), (0, 1), value=-100)[..., 1:]          # position i predicts token i + 1
+        loss = linear_cross_entropy(seen[-1], w, ahead.to(torch.int64))
+        if isinstance(out, tuple):
+            return (loss,) + out[1:]
+        return type(out)(loss=loss, **{k: v for k, v in out.items() if k != "logits"})
+
+
+def use_libofhip_vocab(lm):
+    """Route a Hugging Face causal LM's vocabulary table through libofhip on both ends: the lookup (``embedding_lookup``) and, where labels are
+    given, the loss (``linear_cross_entropy``: the output then has no logits).  Before or after the LM becomes part of a Flamingo."""
+    known = {"MptForCausalLM", "GPTNeoXForCausalLM"}
+    if not known & {c.__name__ for c in type(lm).__mro__}:
+        raise NotImplementedError(f"use_libofhip_vocab knows {sorted(known)}, got {type(lm).__name__}")
+    if isinstance(lm, _VocabLossMixin):
+        return lm
+    emb = lm.get_input_embeddings()
+    if type(emb) is torch.nn.Embedding and emb.max_norm is None and not emb.scale_grad_by_freq and not emb.sparse:
+        emb._of_eager_forward = emb.forward
+        emb.forward = types.MethodType(_embedding_forward, emb)
+    extend_instance(lm, _VocabLossMixin)
+    return lm
