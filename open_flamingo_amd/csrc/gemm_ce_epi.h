@@ -1,12 +1,13 @@
 // Epilogues of the 256x256 GEMM kernel (gemm_w4m.hip) for the loss of a language-model head whose logits are never kept
 // (linear_ce.hip).  Four products of it run on that kernel; a wave owns 128 x 128 of a tile and sends it as eight 32 x 64 groups
 // through its LDS patch (gemm_common.h), so that in a row pass eight lanes hold 8 consecutive columns each of one row:
-//   LSE     z = s x W^T: per row and 128-column strip (max, sum exp(z - max)) -> part[strip][row]; the label's z -> zlab[row].
-//           Statistics in fp32 straight from the fp32 accumulators: a logit is never rounded to bf16.
+//   LSE     z = s x W^T: per row and 128-column strip (max, sum exp(z - max)) -> part[strip][row]; the label's z -> zlab[row], all in units
+//           of log 2.  Statistics in fp32 straight from the fp32 accumulators: a logit is never rounded to bf16.
 //   DLOGIT  the same product again: D = exp(z - lse[row]) - [column == label], times the row's upstream gradient where rows have one of
 //           their own, stored as bf16 (the operand type of the two products behind it; half a unit of 2^-8 of each entry at most).  A
 //           scalar upstream gradient is NOT in D -- it multiplies the fp32 sums of those products instead, so that -1 + p keeps its bits.
-//   DX      dx_acc (fp32) = beta dx_acc + D W over the pieces of the vocabulary
+//   DX      dx_acc (fp32) = beta dx_acc + D W over the pieces of the vocabulary; with few tiles (few rows) the piece is split along the
+//           vocabulary into of_ce_splits parts, each with a dx_acc of its own
 //   DW      dW (bf16) = scale D^T x
 // Rows are the compacted ones (labels that count), padded to 256; the vocabulary's last tile hangs over the table's end: its rows
 // read as zeros (of_buf_make_n), its columns are masked here.
@@ -23,13 +24,14 @@ struct OfCeGemmArgs : OfGemmArgs {      // M, N, K: the padded extents of the la
     int m_valid;             // DW: rows that exist (vocabulary of the piece)
     int col0;                // vocabulary index of column 0 of the piece (labels count from the table's first row)
     const int* lab;          // [row] label, -1 for rows behind `count`
-    const float* lse;        // [row], +inf for rows behind `count`
+    const float* lse;        // [row] in units of log 2, +inf for rows behind `count`
     const float* grow;       // [row] upstream gradient of its own, or NULL
     float* part;             // LSE: [strip][row][2]
     float* zlab;             // LSE: [row]
     long part_ld;            // rows of one strip
     const float* gscale;     // DW: scalar upstream gradient or NULL (1)
     int by_count;            // DW: divide by `count`
+    int split_stages;        // DX: 64-deep stages of a whole piece (the same for every piece: of_ce_splits)
 };
 int of_gemm_w4m_ce(const OfCeGemmArgs& a, of_stream_t s);      // gemm_w4m.hip: a.epi selects the product
 
@@ -42,6 +44,14 @@ template <> struct OfEpiArgs<OF_EPI_CE_DW> { typedef OfCeGemmArgs type; };
 
 // rows a launch works on: at least one tile, so that every product, sum and gradient of a batch without a single label is written (as zeros)
 OF_HOSTDEV int of_ce_live_rows(int count) { return count > 0 ? (count + 255) & ~255 : 256; }
+// Parts a dx product is split into along the vocabulary, so that few rows fill the chip too: 1024 rows x d = 2560 are 40 tiles on 256
+// CUs, 443 us a piece of 32768; as 6 parts 151 us.  A part keeps at least 16 stages of 64 (its prologue and epilogue take about 6).
+OF_HOSTDEV int of_ce_splits(int tiles, int stages) {
+    int s = OF_NUM_CUS / tiles;
+    const int most = stages / 16;
+    if (s > most) s = most;
+    return s < 1 ? 1 : s;
+}
 // the scalar that multiplies both gradients: upstream / number of labels (mean), upstream (sum), 1 (rows have their own)
 OF_DEV float of_ce_scale(const float* gscale, int by_count, const int* count) {
     if (by_count && *count == 0) return 0.f;
@@ -52,11 +62,50 @@ OF_DEV float of_ce_scale(const float* gscale, int by_count, const int* count) {
 namespace oft {
 
 constexpr float CE_LOG2E = 1.4426950408889634f;
+constexpr float CE_LN2 = 0.69314718055994531f;
 constexpr float CE_LOWEST = -3.0e38f;      // the running maximum of nothing: below every finite logit, and no NaN in differences
+
+// LSE straight from the accumulators: lane l of a 16 x 16 fragment holds row l & 15, columns 4 (l >> 4) + 0..3, so that a lane owns 32 of
+// a row's 128 columns in the eight fragments of a row block and the four lanes of a row meet in two register exchanges -- no LDS patch
+// (through it a tile's epilogue took 5 us more of one wave's issue slots).  frag(b) = the row block's fragment of columns 16 b..
+template <class Frag>
+OF_DEV void ce_lse_rows(const OfCeGemmArgs& p, Frag frag, int m_base, int n_base, int lane) {
+    const int m = m_base + (lane & 15), n0 = n_base + 4 * (lane >> 4);
+    const bool edge = n_base + 128 > p.n_valid;
+    const int at = p.lab[m] - p.col0 - n0;            // the label's place counted from this lane's first column
+    const float sc = p.alpha * CE_LOG2E;              // base-2 logits: exp(z - max) is one subtraction and one v_exp_f32
+    float top = CE_LOWEST;
+    f32x4 z[8];
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        z[b] = frag(b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[b][e] *= sc;         // (rounded here: DLOGIT rounds the same product)
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n0 + 16 * b + e >= p.n_valid) z[b][e] = -__builtin_inff();
+        }
+        top = of_max(of_max(top, of_max(z[b][0], z[b][1])), of_max(z[b][2], z[b][3]));
+    }
+    top = of_rows_max(top);
+    float s = 0.f;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) s += (of_exp2(z[b][0] - top) + of_exp2(z[b][1] - top)) + (of_exp2(z[b][2] - top) + of_exp2(z[b][3] - top));
+    s = of_rows_sum(s);
+    if (at >= 0 && at < 116 && (at & 15) < 4) {       // one lane of the row, in one strip
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (at == 16 * b + e) p.zlab[m] = z[b][e];
+    }
+    if (lane < 16) *(f32x2*)(p.part + ((size_t)(n_base >> 7) * p.part_ld + m) * 2) = f32x2{top, s};
+}
 
 // the row passes of one 32 x 64 group (accumulators in the patch)
 template <int EPI>
-OF_DEV void ce_group_rows(const OfCeGemmArgs& p, char* patch, int m_base, int n_base, int lane, float sc, float (&mx)[4], float (&sm)[4]) {
+OF_DEV void ce_group_rows(const OfCeGemmArgs& p, char* patch, int m_base, int n_base, int lane, float sc) {
     constexpr bool SPLIT = EPI == OF_EPI_CE_DX;          // fp32 output: columns 4j.. and 32 + 4j.. (gemm_common.h, epi_split_cols)
     const int hi = SPLIT ? 32 : 4;
     const int rd_row = lane >> 3, rd_col = (lane & 7) * (SPLIT ? 4 : 8);
@@ -66,39 +115,36 @@ OF_DEV void ce_group_rows(const OfCeGemmArgs& p, char* patch, int m_base, int n_
         const int r = it * 8 + rd_row, m = m_base + r, n = n_base + rd_col;
         const f32x4 v0 = *(const f32x4*)(patch + r * ofg::PATCH_PITCH + rd_col * 4), v1 = *(const f32x4*)(patch + r * ofg::PATCH_PITCH + (rd_col + hi) * 4);
         float a[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-        if constexpr (EPI == OF_EPI_CE_LSE || EPI == OF_EPI_CE_DLOGIT) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) a[e] *= sc;
+        if constexpr (EPI == OF_EPI_CE_DLOGIT) {
+            // what few elements need (the label's, columns behind the vocabulary) sits in branches
             const int at = p.lab[m] - p.col0 - n;         // the label's place among this lane's eight columns, if 0 <= at < 8
-            if constexpr (EPI == OF_EPI_CE_LSE) {
-                if (n + 8 > p.n_valid) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (n + e >= p.n_valid) a[e] = -__builtin_inff();
-                }
-                float top = mx[it];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = of_max(top, a[e]);
-                float s = sm[it] * of_exp2((mx[it] - top) * CE_LOG2E);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s += of_exp2((a[e] - top) * CE_LOG2E);
-                mx[it] = top;
-                sm[it] = s;
-                if ((unsigned)at < 8u && n + at < p.n_valid) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (e == at) p.zlab[m] = a[e];
-                }
-            } else {
-                const float l = p.lse[m], g = p.grow ? p.grow[m] : 1.0f;
-                float o[8];
+            const float l = p.lse[m];
+            float o[8];
+            {
+                // the logit as LSE rounded it, then the difference: the same two roundings, so that a row with one class left has p = 1
+                // exactly and no gradient (a fused multiply-add would leave the rounding of lse's own logit in p)
+#pragma clang fp contract(off)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float d = of_exp2((a[e] - l) * CE_LOG2E) - (e == at ? 1.0f : 0.0f);
-                    o[e] = n + e < p.n_valid ? g * d : 0.f;
+                    const float z = a[e] * sc;
+                    o[e] = of_exp2(z - l);
                 }
-                *(u32x4*)((bf16_t*)p.C + (size_t)m * p.ldc + n) = ofg::pack8(o);
             }
+            if ((unsigned)at < 8u) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e == at) o[e] -= 1.0f;
+            }
+            if (p.grow) {
+                const float g = p.grow[m];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] *= g;
+            }
+            if (n_base + 64 > p.n_valid) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = n + e < p.n_valid ? o[e] : 0.f;
+            }
+            *(u32x4*)((bf16_t*)p.C + (size_t)m * p.ldc + n) = ofg::pack8(o);
         } else if constexpr (EPI == OF_EPI_CE_DX) {
             float* c = (float*)p.C + (size_t)m * p.ldc + n;
 #pragma unroll
@@ -129,37 +175,12 @@ template <int EPI, class ToPatch>
 OF_DEV void w4_epilogue_ce(const OfCeGemmArgs& p, ToPatch to_patch, char* smem, int m0, int n0, int wm, int wn, int wave, int lane) {
     char* patch = smem + wave * ofg::PATCH_BYTES;
     float sc = p.alpha;
+    if (EPI == OF_EPI_CE_DLOGIT) sc *= CE_LOG2E;
     if (EPI == OF_EPI_CE_DW) sc *= of_ce_scale(p.gscale, p.by_count, p.count);
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-        float mx[4], sm[4];
-#pragma unroll
-        for (int it = 0; it < 4; ++it) {
-            mx[it] = CE_LOWEST;
-            sm[it] = 0.f;
-        }
-#pragma unroll
-        for (int np = 0; np < 2; ++np) {
-            to_patch(2 * mt + np, patch);
-            ce_group_rows<EPI>(p, patch, m0 + wm * 128 + mt * 32, n0 + wn * 128 + np * 64, lane, sc, mx, sm);
-        }
-        if constexpr (EPI == OF_EPI_CE_LSE) {          // the strip's 128 columns sit in eight lanes: join them, one (max, sum) per row
-#pragma unroll
-            for (int it = 0; it < 4; ++it) {
-#pragma unroll
-                for (int o = 4; o >= 1; o >>= 1) {
-                    const float m2 = of_shfl_xor(mx[it], o), s2 = of_shfl_xor(sm[it], o);
-                    const float top = of_max(mx[it], m2);
-                    sm[it] = sm[it] * of_exp2((mx[it] - top) * CE_LOG2E) + s2 * of_exp2((m2 - top) * CE_LOG2E);
-                    mx[it] = top;
-                }
-                if ((lane & 7) == 0) {
-                    const size_t strip = (size_t)(n0 >> 7) + wn;
-                    const int m = m0 + wm * 128 + mt * 32 + it * 8 + (lane >> 3);
-                    *(f32x2*)(p.part + (strip * p.part_ld + m) * 2) = f32x2{mx[it], sm[it]};
-                }
-            }
-        }
+    for (int g = 0; g < 8; ++g) {
+        to_patch(g, patch);
+        ce_group_rows<EPI>(p, patch, m0 + wm * 128 + (g >> 1) * 32, n0 + wn * 128 + (g & 1) * 64, lane, sc);
     }
 }
 

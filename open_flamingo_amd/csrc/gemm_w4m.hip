@@ -144,11 +144,14 @@ template <bool AT, bool BT, int EPI, bool SK>
 OF_GLOBAL void OF_BOUNDS(256, 1) of_gemm_w4m_kernel(typename OfEpiArgs<EPI>::type p) {
     constexpr bool CE = of_epi_is_ce(EPI);
     static_assert(!CE || !SK, "classic launches only");
+    int parts = 1;                        // DX: parts of K, each on a copy of C of its own
     if constexpr (CE) {
         const int live = of_ce_live_rows(of_uniform(*p.count));
         if (EPI == OF_EPI_CE_DW) p.K = live;
         else p.M = live;
-        if (of_bid_x() >= (p.M / TM) * (p.N / TN)) return;          // (the whole workgroup, in front of every barrier)
+        const int tiles = (p.M / TM) * (p.N / TN);
+        if (EPI == OF_EPI_CE_DX) parts = of_ce_splits(tiles, p.split_stages);
+        if (of_bid_x() >= tiles * parts) return;          // (the whole workgroup, in front of every barrier)
     }
     constexpr bool ASMD = AT || BT;       // LDS-DMA form (of_platform.h): inline asm wherever a transposed-fragment read follows
     OF_STAMP_DECL();
@@ -201,6 +204,14 @@ OF_GLOBAL void OF_BOUNDS(256, 1) of_gemm_w4m_kernel(typename OfEpiArgs<EPI>::typ
             vt = bid;
             s0 = 0;
             nd = nd_all;
+            if constexpr (EPI == OF_EPI_CE_DX) {
+                const int part = bid / ntiles;
+                vt = bid - part * ntiles;
+                s0 = nd_all * part / parts;
+                nd = nd_all * (part + 1) / parts - s0;
+                if (nd == 0) return;      // (a short last piece leaves some parts without a stage; the whole workgroup)
+                p.C = (float*)p.C + (size_t)part * p.M * p.ldc;
+            }
         } else if (seg < rounds) {
             vt = bid + seg * G;
             s0 = 0;
@@ -250,7 +261,7 @@ OF_GLOBAL void OF_BOUNDS(256, 1) of_gemm_w4m_kernel(typename OfEpiArgs<EPI>::typ
         int rot = 0;
         // (only launches of_gemm selected itself: a kernel forced through OfGemmArgs.safe keeps stage order 0, 1, 2, ... -- the order of
         // the general kernel, which the race screens of tests/test_gpu_kernels.py compare with bit for bit)
-        if (p.safe == 0 && (!SK || (s0 == 0 && nd == nd_all))) rot = OF_W4M_ROTATION(vt, bid, pm, pn, tiles_m, tiles_n, nd_all);
+        if (p.safe == 0 && parts == 1 && (!SK || (s0 == 0 && nd == nd_all))) rot = OF_W4M_ROTATION(vt, bid, pm, pn, tiles_m, tiles_n, nd_all);
         int kidx2 = rot + s0 + 1;                                                    // stage index of (sA2, sB2)
         if (kidx2 >= nd_all) kidx2 -= nd_all;
         unsigned sA = (unsigned)(rot + s0) * stepA, sB = (unsigned)(rot + s0) * stepB;          // scalar byte offsets of the next stage to request
@@ -444,7 +455,11 @@ OF_GLOBAL void OF_BOUNDS(256, 1) of_gemm_w4m_kernel(typename OfEpiArgs<EPI>::typ
             }
         };
         // gate-gradient partial of this TILE: slot = its position in the (m-major) tile grid, whichever workgroup finishes it
-        if constexpr (CE) w4_epilogue_ce<EPI>(p, acc_to_patch, smem, m0, n0, wm, wn, wave, lane);
+        if constexpr (EPI == OF_EPI_CE_LSE) {
+#pragma unroll
+            for (int a = 0; a < 8; ++a)
+                ce_lse_rows(p, [&](int b) OF_INLINE_LAMBDA { return acc[a][b]; }, m0 + wm * 128 + a * 16, n0 + wn * 128, lane);
+        } else if constexpr (CE) w4_epilogue_ce<EPI>(p, acc_to_patch, smem, m0, n0, wm, wn, wave, lane);
         else w4_epilogue_with<EPI, ASMD, decltype(acc_to_patch), true, !(EPI == OF_EPI_GATE_RESID && B3)>(p, acc_to_patch, smem, SMEM_W4M, m0, n0, wm, wn, wave, lane, pm * tiles_n + pn);
         OF_STAMP(3);
     }
@@ -507,7 +522,9 @@ int of_gemm_w4m_ce(const OfCeGemmArgs& a, of_stream_t s) {
     const unsigned long long a_span = 2ull * (unsigned long long)(a.a_trans ? a.K : TM) * (unsigned long long)a.lda;
     const unsigned long long b_span = 2ull * (unsigned long long)(a.b_trans ? a.K : TN) * (unsigned long long)a.ldb;
     if (a_span >= (1ull << 32) || b_span >= (1ull << 32)) return OF_E_SHAPE;
-    const of_dim3 grid{(unsigned)((a.M / TM) * (a.N / TN)), 1, 1};
+    // DX: the row count that decides about its parts is on the device; tiles x parts is below the chip's CUs, or the tiles alone
+    const int tiles = (a.M / TM) * (a.N / TN), least = a.epi == OF_EPI_CE_DX && tiles < OF_NUM_CUS ? OF_NUM_CUS : tiles;
+    const of_dim3 grid{(unsigned)least, 1, 1};
     constexpr int smem = SMEM_W4M + OPER_BYTES;
     switch (a.epi) {
         case OF_EPI_CE_LSE: return of_launch(of_gemm_w4m_kernel<false, false, OF_EPI_CE_LSE, false>, grid, 256, smem, s, a);

@@ -14,7 +14,7 @@
 
 namespace {
 
-constexpr int CE_THREADS = 512;
+constexpr int CE_THREADS = 512;          // of the launches that are one workgroup
 
 struct CeRowsArgs {
     const long long* labels; long long ignore_index;
@@ -24,45 +24,61 @@ struct CeRowsArgs {
     const bf16_t* x; long ldx; bf16_t* xc; long ldxc; int d, d_pad;
     const float* part; const float* zlab; long part_ld; int strips;
     float* loss; int mean;
-    const float* grad; int by_count; float logit_scale; const float* acc; long ldacc; bf16_t* dx; long lddx;
+    const float* grad; int by_count; float logit_scale; const float* acc; int split_stages; bf16_t* dx; long lddx;
     float* grow;
     const bf16_t* w; long ldw; bf16_t* wc; long ldwc; long w_rows;
 };
 
 // One workgroup: the rows whose label counts, in order.  slot_of[row] = place among them or -1, row_of its inverse, lab by place;
 // loss_rows of the others is final here: 0 for ignored rows, NaN for a label outside the vocabulary (a caller's mistake that has to
-// surface in the loss; such a row has no gradient).
+// surface in the loss; such a row has no gradient).  A wave owns consecutive 64s of rows: it counts them with one ballot each, the waves'
+// counts are joined, and a second walk over the (cached) labels places them.
 OF_GLOBAL void OF_BOUNDS(CE_THREADS, 1) ce_index_kernel(CeRowsArgs a) {
     int* cum = (int*)of_smem();
-    const int tid = of_tid();
-    const long per = (a.rows + CE_THREADS - 1) / CE_THREADS, lo = tid * per, hi = lo + per < a.rows ? lo + per : a.rows;
+    constexpr int WAVES = CE_THREADS / 64;
+    const int tid = of_tid(), lane = tid & 63, wave = tid >> 6;
+    const long per = ((a.rows + WAVES * 64 - 1) / (WAVES * 64)) * 64, lo = wave * per, hi = lo + per < a.rows ? lo + per : a.rows;
+    auto counts = [&](long r) OF_INLINE_LAMBDA -> bool {
+        if (r >= hi) return false;
+        const long long l = a.labels[r];
+        return l != a.ignore_index && l >= 0 && l < a.vocab;
+    };
     int n = 0;
-    for (long r = lo; r < hi; ++r) {
-        const long long l = a.labels[r];
-        n += l != a.ignore_index && l >= 0 && l < a.vocab;
+    for (long r0 = lo; r0 < lo + per; r0 += 256) {
+        bool c[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) c[u] = counts(r0 + u * 64 + lane);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) n += __builtin_popcountll(of_ballot(c[u]));
     }
-    cum[tid] = n;
+    if (lane == 0) cum[wave] = n;
     of_sync();
-    for (int o = 1; o < CE_THREADS; o <<= 1) {
-        const int v = tid >= o ? cum[tid - o] : 0;
-        of_sync();
-        cum[tid] += v;
-        of_sync();
+    int at = 0, total = 0;
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) at += cum[w];
+        total += cum[w];
     }
-    int at = cum[tid] - n;
-    for (long r = lo; r < hi; ++r) {
-        const long long l = a.labels[r];
-        const bool counts = l != a.ignore_index && l >= 0 && l < a.vocab;
-        a.slot_of[r] = counts ? at : -1;
-        if (counts) {
-            a.row_of[at] = (int)r;
-            a.lab[at] = (int)l;
-            ++at;
-        } else {
-            a.loss_rows[r] = l == a.ignore_index ? 0.f : __builtin_nanf("");
+    for (long r0 = lo; r0 < lo + per; r0 += 256) {
+        long long l[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) l[u] = r0 + u * 64 + lane < hi ? a.labels[r0 + u * 64 + lane] : a.ignore_index;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const long r = r0 + u * 64 + lane;
+            const bool c = r < hi && l[u] != a.ignore_index && l[u] >= 0 && l[u] < a.vocab;
+            const unsigned long long all = of_ballot(c);
+            const int slot = at + __builtin_popcountll(all & ((1ull << lane) - 1));
+            at += __builtin_popcountll(all);
+            if (r >= hi) continue;
+            a.slot_of[r] = c ? slot : -1;
+            if (c) {
+                a.row_of[slot] = (int)r;
+                a.lab[slot] = (int)l[u];
+            } else {
+                a.loss_rows[r] = l[u] == a.ignore_index ? 0.f : __builtin_nanf("");
+            }
         }
     }
-    const int total = cum[CE_THREADS - 1];
     if (tid == 0) *a.count = total;
     for (int i = total + tid; i < of_ce_live_rows(total); i += CE_THREADS) a.lab[i] = -1;
 }
@@ -93,7 +109,7 @@ OF_GLOBAL void OF_BOUNDS(256, 4) ce_pad_table_kernel(CeRowsArgs a) {
         }
 }
 
-// 16 rows a workgroup, 16 lanes a row: lane j joins strips j, j + 16, ... of its row, then the 16 lanes in a fixed order
+// 16 rows a workgroup, 16 lanes a row: lane j joins strips j, j + 16, ... of its row, then the 16 lanes in a fixed order (base-2 logits)
 OF_GLOBAL void OF_BOUNDS(256, 2) ce_finish_kernel(CeRowsArgs a) {
     float* red = (float*)of_smem();          // [16 groups][16 rows][2]
     const int tid = of_tid(), r = tid & 15, j = tid >> 4, count = *a.count;
@@ -101,10 +117,11 @@ OF_GLOBAL void OF_BOUNDS(256, 2) ce_finish_kernel(CeRowsArgs a) {
     if (i0 >= of_ce_live_rows(count)) return;
     const long i = i0 + r;
     float m = oft::CE_LOWEST, s = 0.f;
+#pragma unroll 4
     for (int t = j; t < a.strips; t += 16) {
         const f32x2 q = *(const f32x2*)(a.part + ((size_t)t * a.part_ld + i) * 2);
         const float top = of_max(m, q[0]);
-        s = s * of_exp2((m - top) * oft::CE_LOG2E) + q[1] * of_exp2((q[0] - top) * oft::CE_LOG2E);
+        s = s * of_exp2(m - top) + q[1] * of_exp2(q[0] - top);
         m = top;
     }
     red[(j * 16 + r) * 2] = m;
@@ -114,10 +131,10 @@ OF_GLOBAL void OF_BOUNDS(256, 2) ce_finish_kernel(CeRowsArgs a) {
         float top = red[r * 2];
         for (int k = 1; k < 16; ++k) top = of_max(top, red[(k * 16 + r) * 2]);
         float sum = 0.f;
-        for (int k = 0; k < 16; ++k) sum += red[(k * 16 + r) * 2 + 1] * of_exp2((red[(k * 16 + r) * 2] - top) * oft::CE_LOG2E);
-        const float lse = top + of_log2(sum) * 0.69314718055994531f;
+        for (int k = 0; k < 16; ++k) sum += red[(k * 16 + r) * 2 + 1] * of_exp2(red[(k * 16 + r) * 2] - top);
+        const float lse = top + of_log2(sum);
         a.lse[i] = i < count ? lse : __builtin_inff();          // behind `count`: exp(z - inf) = 0, rows of D that are zero
-        if (i < count) a.loss_rows[a.row_of[i]] = lse - a.zlab[i];
+        if (i < count) a.loss_rows[a.row_of[i]] = (lse - a.zlab[i]) * oft::CE_LN2;
     }
 }
 
@@ -143,24 +160,30 @@ OF_GLOBAL void OF_BOUNDS(256, 4) ce_row_grads_kernel(CeRowsArgs a) {
     if (i < of_ce_live_rows(count)) a.grow[i] = i < count ? a.grad[a.row_of[i]] : 0.f;
 }
 
-// dx[row] = bf16(logit_scale * scale * acc[place]), zeros for rows without a label; one wave per row
+// dx[row] = bf16(logit_scale * scale * the sum of acc's parts), zeros for rows without a label; one wave per row
 OF_GLOBAL void OF_BOUNDS(256, 4) ce_scatter_kernel(CeRowsArgs a) {
     const int lane = of_tid() & 63;
     const long r = (long)of_bid_x() * 4 + (of_tid() >> 6);
     if (r >= a.rows) return;
-    const int i = a.slot_of[r];
+    const int i = a.slot_of[r], live = of_ce_live_rows(*a.count);
+    const int parts = of_ce_splits((live >> 8) * ((a.d + 255) >> 8), a.split_stages);
+    const size_t part = (size_t)live * a.d;
     const float sc = a.logit_scale * of_ce_scale(a.grad, a.by_count, a.count);
-    const float* src = i < 0 ? nullptr : a.acc + (size_t)i * a.ldacc;
+    const float* src = i < 0 ? nullptr : a.acc + (size_t)i * a.d;
     bf16_t* dst = a.dx + (size_t)r * a.lddx;
     for (int c = lane * 8; c < a.d; c += 512) {
         float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (src) {
-            const f32x4 v0 = *(const f32x4*)(src + c), v1 = *(const f32x4*)(src + c + 4);
+            for (int k = 0; k < parts; ++k) {
+                const f32x4 v0 = *(const f32x4*)(src + k * part + c), v1 = *(const f32x4*)(src + k * part + c + 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                o[e] = sc * v0[e];
-                o[4 + e] = sc * v1[e];
+                for (int e = 0; e < 4; ++e) {
+                    o[e] += v0[e];
+                    o[4 + e] += v1[e];
+                }
             }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] *= sc;
         }
         *(u32x4*)(dst + c) = ofg::pack8(o);
     }
@@ -205,6 +228,13 @@ int ce_piece(const OfLinearCeArgs& a) {
     const long all = (a.vocab + 255l) & ~255l;
     if (p < 256) p = 256;
     return (int)(p < all ? p : all);
+}
+// fp32 sums of dx: rows x d, or the parts of fewer rows (of_ce_splits: parts x tiles <= the chip's CUs)
+size_t ce_acc_bytes(const OfLinearCeArgs& a) {
+    const long rp = rows_padded(a.rows), nt = (a.d + 255) >> 8, most = ce_piece(a) / 64 / 16;
+    long rows = OF_NUM_CUS / nt * 256;
+    if (rows > most * rp) rows = most * rp;
+    return up256((size_t)(rows > rp ? rows : rp) * a.d * 4);
 }
 size_t ce_table_bytes(const OfLinearCeArgs& a) { return depth_padded(a.d) != a.d ? up256((size_t)a.vocab * depth_padded(a.d) * 2) : 0; }
 
@@ -264,7 +294,7 @@ extern "C" size_t of_linear_ce_workspace_bytes(const OfLinearCeArgs* args, int b
     const OfLinearCeArgs& a = *args;
     const size_t rp = (size_t)rows_padded(a.rows);
     if (!backward) return ce_table_bytes(a) + up256((size_t)(((a.vocab + 255l) / 256) * 2) * rp * 8) + up256(rp * 4);
-    return ce_table_bytes(a) + up256(rp * (size_t)ce_piece(a) * 2) + (a.dx ? up256(rp * (size_t)a.d * 4) : 0) + (a.reduction == OF_CE_NONE ? up256(rp * 4) : 0);
+    return ce_table_bytes(a) + up256(rp * (size_t)ce_piece(a) * 2) + (a.dx ? ce_acc_bytes(a) : 0) + (a.reduction == OF_CE_NONE ? up256(rp * 4) : 0);
 }
 
 extern "C" int of_linear_ce_fwd(const OfLinearCeArgs* args, void* stream) {
@@ -329,12 +359,12 @@ extern "C" int of_linear_ce_bwd(const OfLinearCeArgs* args, void* stream) {
     float* acc = nullptr;
     if (a.dx) {
         acc = (float*)ws;
-        ws += up256((size_t)rp * a.d * 4);
+        ws += ce_acc_bytes(a);
     }
 
     CeRowsArgs r{};
     r.rows = a.rows; r.count = st.count; r.slot_of = st.slot_of; r.row_of = st.row_of;
-    r.d = a.d; r.acc = acc; r.ldacc = a.d; r.dx = a.dx; r.lddx = a.lddx;
+    r.d = a.d; r.acc = acc; r.split_stages = piece / 64; r.dx = a.dx; r.lddx = a.lddx;
     if (a.reduction == OF_CE_NONE) {
         r.grad = a.grad;
         r.grow = (float*)ws;
@@ -359,7 +389,7 @@ extern "C" int of_linear_ce_bwd(const OfLinearCeArgs* args, void* stream) {
             q.b_bytes = ((long)(n - 1) * ldw + dp) * 2;
             q.M = (int)rp; q.N = d256; q.K = (n + 63) & ~63;
             q.C = acc; q.ldc = a.d; q.beta = v0 ? 1.f : 0.f; q.alpha = 1.f;
-            q.count = st.count; q.n_valid = a.d;
+            q.count = st.count; q.n_valid = a.d; q.split_stages = piece / 64;
             rc = of_gemm_w4m_ce(q, s);
             if (rc) return rc;
         }
