@@ -381,9 +381,10 @@ int of_ce_bwd(const void* logits, int logits_f32, long ld, const long long* labe
  *              vocabulary, get zeros and add nothing.  The same x, w, labels, rows, vocab, d, logit_scale and reduction as the forward.
  *              The vocabulary is walked in pieces of `piece` rows (rounded down to a multiple of 256, at least 256; 0: chosen so that a
  *              piece of the logits' gradient, rows x piece bf16, takes 128 MB).
+ *              of_linear_ce_stateless(rows, d) = 1 (a handful of rows: scoring next tokens): `state` may be NULL, with no backward to follow
  * Deterministic: no atomics.  d % 8 == 0; x, w, dx, dw 16-byte aligned like state and workspace, row strides
- * multiples of 8.  The workspace holds of_linear_ce_workspace_bytes(args, backward) bytes: the fields rows, vocab, d, piece, reduction and
- * (backward) dx of args decide. */
+ * multiples of 8.  The workspace holds of_linear_ce_workspace_bytes(args, backward) bytes: the fields rows, vocab, d, piece, reduction,
+ * state and (backward) dx of args decide. */
 enum { OF_CE_NONE = 0, OF_CE_MEAN = 1, OF_CE_SUM = 2 };
 typedef struct OfLinearCeArgs {
     const uint16_t* x; long ldx;
@@ -403,6 +404,7 @@ typedef struct OfLinearCeArgs {
     void* workspace; size_t workspace_bytes;
 } OfLinearCeArgs;
 size_t of_linear_ce_state_bytes(long rows, int d);
+int of_linear_ce_stateless(long rows, int d);
 size_t of_linear_ce_workspace_bytes(const OfLinearCeArgs* args, int backward);
 int of_linear_ce_fwd(const OfLinearCeArgs* args, void* stream);
 int of_linear_ce_bwd(const OfLinearCeArgs* args, void* stream);

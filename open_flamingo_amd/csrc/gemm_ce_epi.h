@@ -45,10 +45,11 @@ template <> struct OfEpiArgs<OF_EPI_CE_DW> { typedef OfCeGemmArgs type; };
 // rows a launch works on: at least one tile, so that every product, sum and gradient of a batch without a single label is written (as zeros)
 OF_HOSTDEV int of_ce_live_rows(int count) { return count > 0 ? (count + 255) & ~255 : 256; }
 // Parts a dx product is split into along the vocabulary, so that few rows fill the chip too: 1024 rows x d = 2560 are 40 tiles on 256
-// CUs, 443 us a piece of 32768; as 6 parts 151 us.  A part keeps at least 16 stages of 64 (its prologue and epilogue take about 6).
+// CUs, 443 us a piece of 32768; as 6 parts 151 us.  A part keeps at least 4 stages of 64.
+constexpr int CE_PART_STAGES = 4;
 OF_HOSTDEV int of_ce_splits(int tiles, int stages) {
     int s = OF_NUM_CUS / tiles;
-    const int most = stages / 16;
+    const int most = stages / CE_PART_STAGES;
     if (s > most) s = most;
     return s < 1 ? 1 : s;
 }

@@ -98,6 +98,52 @@ OF_GLOBAL void OF_BOUNDS(256, 4) ce_gather_kernel(CeRowsArgs a) {
     }
 }
 
+// Both of the above in one launch for at most 1024 rows: every wave finds its place's row by counting the labels itself (16 ballots), the
+// first workgroup also writes the lists.
+constexpr int CE_FEW_ROWS = 1024;
+OF_GLOBAL void OF_BOUNDS(256, 4) ce_index_gather_kernel(CeRowsArgs a) {
+    const int lane = of_tid() & 63, wave = of_tid() >> 6, rows = (int)a.rows;
+    const int i = of_bid_x() * 4 + wave;
+    int at = 0, mine = -1;
+    for (int r0 = 0; r0 < rows; r0 += 256) {
+        long long l[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) l[u] = r0 + u * 64 + lane < rows ? a.labels[r0 + u * 64 + lane] : a.ignore_index;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = r0 + u * 64 + lane;
+            const bool c = l[u] != a.ignore_index && l[u] >= 0 && l[u] < a.vocab;
+            const unsigned long long all = of_ballot(c);
+            const int slot = at + __builtin_popcountll(all & ((1ull << lane) - 1));
+            const unsigned long long hit = of_ballot(c && slot == i);
+            if (hit) mine = r0 + u * 64 + __builtin_ctzll(hit);
+            at += __builtin_popcountll(all);
+            if (of_bid_x() == 0 && wave == 0 && r < rows) {
+                a.slot_of[r] = c ? slot : -1;
+                if (c) {
+                    a.row_of[slot] = r;
+                    a.lab[slot] = (int)l[u];
+                } else {
+                    a.loss_rows[r] = l[u] == a.ignore_index ? 0.f : __builtin_nanf("");
+                }
+            }
+        }
+    }
+    const int live = of_ce_live_rows(at);
+    if (of_bid_x() == 0 && wave == 0) {
+        if (lane == 0) *a.count = at;
+        for (int k = at + lane; k < live; k += 64) a.lab[k] = -1;
+    }
+    if (i >= live) return;
+    const bf16_t* src = mine >= 0 ? a.x + (size_t)mine * a.ldx : nullptr;
+    bf16_t* dst = a.xc + (size_t)i * a.ldxc;
+    for (int c = lane * 8; c < a.d_pad; c += 512) {
+        u32x4 v = {0u, 0u, 0u, 0u};
+        if (src && c < a.d) v = *(const u32x4*)(src + c);
+        *(u32x4*)(dst + c) = v;
+    }
+}
+
 // the table with its rows padded to a multiple of 64 columns by zeros (only where d is none)
 OF_GLOBAL void OF_BOUNDS(256, 4) ce_pad_table_kernel(CeRowsArgs a) {
     const int lane = of_tid() & 63;
@@ -151,6 +197,176 @@ OF_GLOBAL void OF_BOUNDS(CE_THREADS, 1) ce_reduce_kernel(CeRowsArgs a) {
         of_sync();
     }
     if (tid == 0) *a.loss = a.mean ? red[0] / (float)*a.count : red[0];
+}
+
+// both of the above in one workgroup where there is little to join
+constexpr int CE_FEW_PARTS = 1 << 14;
+OF_GLOBAL void OF_BOUNDS(CE_THREADS, 1) ce_finish_reduce_kernel(CeRowsArgs a) {
+    float* red = (float*)of_smem();
+    const int tid = of_tid(), count = *a.count, live = of_ce_live_rows(count);
+    float sum = 0.f;
+    for (int i = tid; i < live; i += CE_THREADS) {
+        float m = oft::CE_LOWEST, s = 0.f;
+#pragma unroll 4
+        for (int t = 0; t < a.strips; ++t) {
+            const f32x2 q = *(const f32x2*)(a.part + ((size_t)t * a.part_ld + i) * 2);
+            const float top = of_max(m, q[0]);
+            s = s * of_exp2(m - top) + q[1] * of_exp2(q[0] - top);
+            m = top;
+        }
+        const float lse = m + of_log2(s);
+        a.lse[i] = i < count ? lse : __builtin_inff();
+        if (i < count) {
+            const float l = (lse - a.zlab[i]) * oft::CE_LN2;
+            a.loss_rows[a.row_of[i]] = l;
+            sum += l;
+        }
+    }
+    if (!a.loss) return;
+    for (long r = tid; r < a.rows; r += CE_THREADS)
+        if (a.slot_of[r] < 0) sum += a.loss_rows[r];          // zeros, and the NaN of a label outside the vocabulary
+    red[tid] = sum;
+    of_sync();
+    for (int o = CE_THREADS / 2; o >= 1; o >>= 1) {
+        if (tid < o) red[tid] += red[tid + o];
+        of_sync();
+    }
+    if (tid == 0) *a.loss = a.mean ? red[0] / (float)count : red[0];
+}
+
+// ------------------------------------------------------------------------------------------------ a handful of rows, no gradient
+// Scoring the next token of up to 16 sequences: the table is read once and nothing else counts (206 MB at 50435 x 2048: 40 us at the
+// rate of a large copy), while a 256-row MFMA tile would be 1/16 ... 1/256 full.  A wave takes four table rows at a time, 16 bytes a lane and
+// row, against the rows of x in LDS (v_dot2, fp32); a halving butterfly leaves every (row, table row) product in a lane of its own, which
+// keeps that pair's running maximum and sum.
+constexpr int FEW_WAVES = 4, FEW_R = 4, FEW_WG = 512;
+struct CeFewArgs {
+    const bf16_t* x; long ldx; const bf16_t* w; long ldw; const long long* labels; long long ignore_index;
+    int rows, vocab, d; float scale;          // scale: logit_scale * log2 e
+    float* part; float* zlab; float* loss_rows; float* loss; int mean;
+};
+template <int MT>
+OF_GLOBAL void OF_BOUNDS(FEW_WAVES * 64, 2) ce_few_kernel(CeFewArgs a) {
+    constexpr int V = MT * FEW_R;
+    const int tid = of_tid(), lane = tid & 63, wave = tid >> 6;
+    bf16_t* xs = (bf16_t*)of_smem();                                   // [MT][d]
+    float* red = (float*)(of_smem() + (((size_t)MT * a.d * 2 + 15) & ~(size_t)15));      // [FEW_WAVES][V][2]
+    for (int i = tid * 8; i < MT * a.d; i += FEW_WAVES * 64 * 8) {
+        const int m = i / a.d, k = i - m * a.d;
+        *(u32x4*)(xs + i) = m < a.rows ? *(const u32x4*)(a.x + (size_t)m * a.ldx + k) : u32x4{0u, 0u, 0u, 0u};
+    }
+    of_sync();
+    // the pair this lane ends up with (the same every time) and its label
+    int pair = 0;
+    {
+        int live = V;
+#pragma unroll
+        for (int s = 0; s < 6; ++s)
+            if (live > 1) {
+                live >>= 1;
+                pair += ((lane >> s) & 1) * live;
+            }
+    }
+    const int m = pair / FEW_R;
+    const long long lab = m < a.rows ? a.labels[m] : -1;
+    float top = oft::CE_LOWEST, sum = 0.f;
+    const int groups = (a.vocab + FEW_R - 1) / FEW_R;
+    for (int g = of_bid_x() * FEW_WAVES + wave; g < groups; g += FEW_WG * FEW_WAVES) {
+        const int n0 = g * FEW_R;
+        float acc[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = 0.f;
+#pragma unroll 4
+        for (int k = lane * 8; k < a.d; k += 512) {
+            u32x4 w[FEW_R];
+#pragma unroll
+            for (int r = 0; r < FEW_R; ++r) {
+                const int n = n0 + r < a.vocab ? n0 + r : a.vocab - 1;          // (computed and dropped)
+                w[r] = *(const u32x4*)(a.w + (size_t)n * a.ldw + k);
+            }
+#pragma unroll
+            for (int mm = 0; mm < MT; ++mm) {
+                const u32x4 x = *(const u32x4*)(xs + mm * a.d + k);
+#pragma unroll
+                for (int r = 0; r < FEW_R; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[mm * FEW_R + r] = of_dot2_bf16(x[e], w[r][e], acc[mm * FEW_R + r]);
+            }
+        }
+        int live = V;
+#pragma unroll
+        for (int s = 0; s < 6; ++s) {
+            const int bit = (lane >> s) & 1;
+            if (live > 1) {
+                live >>= 1;
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i)
+                    if (i < live) {
+                        const float lo = acc[i], hi = acc[i + live];
+                        acc[i] = (bit ? hi : lo) + of_shfl_xor(bit ? lo : hi, 1 << s);
+                    }
+            } else {
+                acc[0] += of_shfl_xor(acc[0], 1 << s);
+            }
+        }
+        const int n = n0 + pair % FEW_R;
+        if (n < a.vocab) {
+            const float z = acc[0] * a.scale, t = of_max(top, z);
+            sum = sum * of_exp2(top - t) + of_exp2(z - t);
+            top = t;
+            if (n == lab) a.zlab[m] = z;
+        }
+    }
+    if (lane < V) {
+        red[(wave * V + pair) * 2] = top;
+        red[(wave * V + pair) * 2 + 1] = sum;
+    }
+    of_sync();
+    if (tid < a.rows) {
+        float t = oft::CE_LOWEST, s = 0.f;
+        for (int i = 0; i < FEW_WAVES * FEW_R; ++i) {
+            const float* q = red + ((i / FEW_R) * V + tid * FEW_R + i % FEW_R) * 2;
+            const float u = of_max(t, q[0]);
+            s = s * of_exp2(t - u) + q[1] * of_exp2(q[0] - u);
+            t = u;
+        }
+        *(f32x2*)(a.part + ((size_t)tid * FEW_WG + of_bid_x()) * 2) = f32x2{t, s};
+    }
+}
+// one workgroup, a wave at a time per row: the 512 partial results of a row, its loss, and their sum
+OF_GLOBAL void OF_BOUNDS(256, 1) ce_few_finish_kernel(CeFewArgs a) {
+    float* red = (float*)of_smem();
+    const int tid = of_tid(), lane = tid & 63, wave = tid >> 6;
+    for (int m = wave; m < a.rows; m += 4) {
+        f32x2 q[FEW_WG / 64];
+#pragma unroll
+        for (int u = 0; u < FEW_WG / 64; ++u) q[u] = *(const f32x2*)(a.part + ((size_t)m * FEW_WG + u * 64 + lane) * 2);
+        float top = oft::CE_LOWEST;
+#pragma unroll
+        for (int u = 0; u < FEW_WG / 64; ++u) top = of_max(top, q[u][0]);
+        top = of_wave_max(top);
+        float s = 0.f;
+#pragma unroll
+        for (int u = 0; u < FEW_WG / 64; ++u) s += q[u][1] * of_exp2(q[u][0] - top);
+        s = of_wave_sum(s);
+        if (lane == 0) {
+            const long long l = a.labels[m];
+            const float lse = top + of_log2(s);
+            const float loss = l == a.ignore_index ? 0.f : l >= 0 && l < a.vocab ? (lse - a.zlab[m]) * oft::CE_LN2 : __builtin_nanf("");
+            a.loss_rows[m] = loss;
+            red[m] = loss;
+        }
+    }
+    of_sync();
+    if (tid == 0 && a.loss) {
+        float sum = 0.f;
+        int n = 0;
+        for (int m = 0; m < a.rows; ++m) {
+            sum += red[m];
+            n += a.labels[m] != a.ignore_index;
+        }
+        *a.loss = a.mean ? sum / (float)n : sum;
+    }
 }
 
 // upstream gradients of the rows, by place
@@ -231,22 +447,25 @@ int ce_piece(const OfLinearCeArgs& a) {
 }
 // fp32 sums of dx: rows x d, or the parts of fewer rows (of_ce_splits: parts x tiles <= the chip's CUs)
 size_t ce_acc_bytes(const OfLinearCeArgs& a) {
-    const long rp = rows_padded(a.rows), nt = (a.d + 255) >> 8, most = ce_piece(a) / 64 / 16;
+    const long rp = rows_padded(a.rows), nt = (a.d + 255) >> 8, most = ce_piece(a) / 64 / CE_PART_STAGES;
     long rows = OF_NUM_CUS / nt * 256;
     if (rows > most * rp) rows = most * rp;
     return up256((size_t)(rows > rp ? rows : rp) * a.d * 4);
 }
 size_t ce_table_bytes(const OfLinearCeArgs& a) { return depth_padded(a.d) != a.d ? up256((size_t)a.vocab * depth_padded(a.d) * 2) : 0; }
 
-int ce_check(const OfLinearCeArgs* args) {
+bool ce_few(long rows, int d) { return rows > 0 && rows <= 16 && d > 0 && (d & 7) == 0 && rows * d <= 1 << 15; }          // (rounded up: 128 KB of x in LDS at most)
+
+int ce_check(const OfLinearCeArgs* args, bool few = false) {
     if (!args) return OF_E_ARG;
     const OfLinearCeArgs& a = *args;
-    if (!a.x || !a.w || !a.labels || !a.state || !a.workspace) return OF_E_ARG;
+    if (!a.x || !a.w || !a.labels || (!a.state && !few) || !a.workspace) return OF_E_ARG;
     if (a.rows <= 0 || a.vocab <= 0 || a.d <= 0 || a.ldx < a.d || a.ldw < a.d || a.piece < 0) return OF_E_ARG;
     if (a.reduction < OF_CE_NONE || a.reduction > OF_CE_SUM) return OF_E_ARG;
     if ((a.d & 7) || a.rows > (1l << 30) || a.vocab > (1 << 30)) return OF_E_SHAPE;
     if ((a.ldx & 7) || (a.ldw & 7) || ((uintptr_t)a.x & 15) || ((uintptr_t)a.w & 15) || ((uintptr_t)a.state & 15) || ((uintptr_t)a.workspace & 15))
         return OF_E_ALIGN;
+    if (few) return 0;
     if (a.state_bytes < of_linear_ce_state_bytes(a.rows, a.d)) return OF_E_WORKSPACE;
     // byte offsets inside a tile's operand windows are 32-bit (gemm_w4m.hip); the weight gradient walks all rows of D and of xc
     const unsigned long long lim = 1ull << 32;
@@ -289,18 +508,41 @@ OfCeGemmArgs ce_logits_args(const OfLinearCeArgs& a, const CeState& st, const bf
 
 extern "C" size_t of_linear_ce_state_bytes(long rows, int d) { return rows > 0 && d > 0 ? ce_state(nullptr, rows, d).bytes : 0; }
 
+extern "C" int of_linear_ce_stateless(long rows, int d) { return ce_few(rows, d); }
+
 extern "C" size_t of_linear_ce_workspace_bytes(const OfLinearCeArgs* args, int backward) {
     if (!args || args->rows <= 0 || args->vocab <= 0 || args->d <= 0) return 0;
     const OfLinearCeArgs& a = *args;
     const size_t rp = (size_t)rows_padded(a.rows);
+    if (!backward && !a.state && ce_few(a.rows, a.d)) return (size_t)a.rows * FEW_WG * 8 + 256;
     if (!backward) return ce_table_bytes(a) + up256((size_t)(((a.vocab + 255l) / 256) * 2) * rp * 8) + up256(rp * 4);
     return ce_table_bytes(a) + up256(rp * (size_t)ce_piece(a) * 2) + (a.dx ? ce_acc_bytes(a) : 0) + (a.reduction == OF_CE_NONE ? up256(rp * 4) : 0);
 }
 
+template <int MT>
+static int ce_few_launch(const CeFewArgs& f, of_stream_t s) {
+    const size_t lds = (((size_t)MT * f.d * 2 + 15) & ~(size_t)15) + FEW_WAVES * MT * FEW_R * 2 * sizeof(float);
+    const int rc = of_launch(ce_few_kernel<MT>, of_dim3{FEW_WG, 1, 1}, FEW_WAVES * 64, lds, s, f);
+    return rc ? rc : of_launch(ce_few_finish_kernel, of_dim3{1, 1, 1}, 256, 16 * sizeof(float), s, f);
+}
+
 extern "C" int of_linear_ce_fwd(const OfLinearCeArgs* args, void* stream) {
-    const int bad = ce_check(args);
+    const bool few = args && !args->state && ce_few(args->rows, args->d);
+    const int bad = ce_check(args, few);
     if (bad) return bad;
     const OfLinearCeArgs& a = *args;
+    if (few) {
+        if (!a.loss_rows || (a.reduction != OF_CE_NONE && !a.loss)) return OF_E_ARG;
+        if (a.workspace_bytes < of_linear_ce_workspace_bytes(args, 0)) return OF_E_WORKSPACE;
+        CeFewArgs f{a.x, a.ldx, a.w, a.ldw, a.labels, a.ignore_index, (int)a.rows, a.vocab, a.d, a.logit_scale * oft::CE_LOG2E, (float*)((char*)a.workspace + 256),
+                    (float*)a.workspace, a.loss_rows, a.reduction == OF_CE_NONE ? nullptr : a.loss, a.reduction == OF_CE_MEAN};
+        of_stream_t s = (of_stream_t)stream;
+        if (a.rows <= 1) return ce_few_launch<1>(f, s);
+        if (a.rows <= 2) return ce_few_launch<2>(f, s);
+        if (a.rows <= 4) return ce_few_launch<4>(f, s);
+        if (a.rows <= 8) return ce_few_launch<8>(f, s);
+        return ce_few_launch<16>(f, s);
+    }
     if (!a.loss_rows || (a.reduction != OF_CE_NONE && !a.loss)) return OF_E_ARG;
     if (a.workspace_bytes < of_linear_ce_workspace_bytes(args, 0)) return OF_E_WORKSPACE;
     of_stream_t s = (of_stream_t)stream;
@@ -315,11 +557,15 @@ extern "C" int of_linear_ce_fwd(const OfLinearCeArgs* args, void* stream) {
     CeRowsArgs r{};
     r.labels = a.labels; r.ignore_index = a.ignore_index; r.rows = a.rows; r.vocab = a.vocab;
     r.count = st.count; r.slot_of = st.slot_of; r.row_of = st.row_of; r.lab = st.lab; r.lse = st.lse;
-    r.loss_rows = a.loss_rows; r.loss = a.loss; r.mean = a.reduction == OF_CE_MEAN;
+    r.loss_rows = a.loss_rows; r.loss = a.reduction == OF_CE_NONE ? nullptr : a.loss; r.mean = a.reduction == OF_CE_MEAN;
     r.x = a.x; r.ldx = a.ldx; r.xc = st.xc; r.ldxc = depth_padded(a.d); r.d = a.d; r.d_pad = depth_padded(a.d);
-    rc = of_launch(ce_index_kernel, of_dim3{1, 1, 1}, CE_THREADS, CE_THREADS * sizeof(int), s, r);
-    if (rc) return rc;
-    rc = of_launch(ce_gather_kernel, of_dim3{(unsigned)(rp / 4), 1, 1}, 256, 0, s, r);
+    if (a.rows <= CE_FEW_ROWS) {
+        rc = of_launch(ce_index_gather_kernel, of_dim3{(unsigned)(rp / 4), 1, 1}, 256, 0, s, r);
+    } else {
+        rc = of_launch(ce_index_kernel, of_dim3{1, 1, 1}, CE_THREADS, CE_THREADS / 64 * sizeof(int), s, r);
+        if (rc) return rc;
+        rc = of_launch(ce_gather_kernel, of_dim3{(unsigned)(rp / 4), 1, 1}, 256, 0, s, r);
+    }
     if (rc) return rc;
 
     OfCeGemmArgs g = ce_logits_args(a, st, w, ldw, 0, a.vocab);
@@ -330,6 +576,7 @@ extern "C" int of_linear_ce_fwd(const OfLinearCeArgs* args, void* stream) {
     rc = of_gemm_w4m_ce(g, s);
     if (rc) return rc;
     r.part = g.part; r.part_ld = rp; r.zlab = g.zlab;
+    if (rp * r.strips <= CE_FEW_PARTS) return of_launch(ce_finish_reduce_kernel, of_dim3{1, 1, 1}, CE_THREADS, CE_THREADS * sizeof(float), s, r);
     rc = of_launch(ce_finish_kernel, of_dim3{(unsigned)(rp / 16), 1, 1}, 256, 16 * 16 * 2 * sizeof(float), s, r);
     if (rc || a.reduction == OF_CE_NONE) return rc;
     return of_launch(ce_reduce_kernel, of_dim3{1, 1, 1}, CE_THREADS, CE_THREADS * sizeof(float), s, r);

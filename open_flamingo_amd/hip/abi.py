@@ -157,6 +157,7 @@ PROTOTYPES = {
     "of_ce_fwd": (C.c_int, [vp, C.c_int, C.c_long, vp, C.c_longlong, C.c_long, C.c_int, vp, vp, vp]),
     "of_ce_bwd": (C.c_int, [vp, C.c_int, C.c_long, vp, C.c_longlong, C.c_long, C.c_int, vp, vp, vp, C.c_long, vp]),
     "of_linear_ce_state_bytes": (C.c_size_t, [C.c_long, C.c_int]),
+    "of_linear_ce_stateless": (C.c_int, [C.c_long, C.c_int]),
     "of_linear_ce_workspace_bytes": (C.c_size_t, [C.POINTER(OfLinearCeArgs), C.c_int]),
     "of_linear_ce_fwd": (C.c_int, [C.POINTER(OfLinearCeArgs), vp]),
     "of_linear_ce_bwd": (C.c_int, [C.POINTER(OfLinearCeArgs), vp]),

@@ -48,7 +48,8 @@ class Ops:
         if cls._default is None:
             from . import lib as _lib
             handle = _lib.load()
-            cls._default = cls(handle, lambda: torch.cuda.current_stream().cuda_stream)
+            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)          # the same handle without a Stream object (2.8 -> 0.5 us a launch)
+            cls._default = cls(handle, (lambda: raw(torch.cuda.current_device())) if raw is not None else (lambda: torch.cuda.current_stream().cuda_stream))
         return cls._default
 
     def _stream(self):
@@ -459,14 +460,15 @@ class Ops:
             raise ValueError(f"hidden states {tuple(x.shape)} and table {tuple(w.shape)} do not fit")
         if labels.dtype != torch.int64 or not labels.is_contiguous() or labels.numel() != rows:
             raise ValueError("labels: one int64 per row, contiguous")
-        assert x.stride(1) == 1 and w.stride(1) == 1 and state.dtype == torch.uint8 and state.is_contiguous()
+        assert x.stride(1) == 1 and w.stride(1) == 1 and (state is None or (state.dtype == torch.uint8 and state.is_contiguous()))
         a = abi.OfLinearCeArgs()
         a.x, a.ldx = x.data_ptr(), x.stride(0) if rows > 1 else max(x.stride(0), d)
         a.w, a.ldw = w.data_ptr(), w.stride(0) if w.shape[0] > 1 else max(w.stride(0), d)
         a.labels, a.ignore_index = labels.data_ptr(), ignore_index
         a.rows, a.vocab, a.d = rows, w.shape[0], d
         a.logit_scale, a.reduction, a.piece = logit_scale, reduction, piece
-        a.state, a.state_bytes = state.data_ptr(), state.numel()
+        if state is not None:
+            a.state, a.state_bytes = state.data_ptr(), state.numel()
         return a
 
     def _linear_ce_workspace(self, a, backward, device):
@@ -474,8 +476,10 @@ class Ops:
         a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
         return ws
 
-    def linear_ce_state(self, rows, d, device):
-        """what linear_ce_fwd leaves for linear_ce_bwd (of_linear_ce_state_bytes)"""
+    def linear_ce_state(self, rows, d, device, grad=True):
+        """what linear_ce_fwd leaves for linear_ce_bwd (of_linear_ce_state_bytes); grad = False, no backward to follow: None where none is needed"""
+        if not grad and self.lib.of_linear_ce_stateless(rows, d):
+            return None
         return torch.empty(self.lib.of_linear_ce_state_bytes(rows, d), dtype=torch.uint8, device=device)
 
     def linear_ce_fwd(self, x, w, labels, state, loss_rows, loss=None, *, ignore_index=-100, logit_scale=1.0, reduction=abi.CE_MEAN):
@@ -503,11 +507,14 @@ class Ops:
     # ------------------------------------------------------------------ lookup in a vocabulary table
     def embedding_fwd(self, ids, table, out, scale=1.0):
         """out[i] = scale * table[ids[i]] (fp32 or bf16 like the table); NaN rows for ids outside it."""
-        assert ids.dtype == torch.int64 and ids.dim() == 1 and ids.is_contiguous() and out.dtype == table.dtype
-        assert out.shape == (ids.numel(), table.shape[1]) and table.stride(1) == 1 and out.stride(1) == 1
-        d = table.shape[1]
-        self._chk(self.lib.of_embedding_fwd(ids.data_ptr(), ids.numel(), table.data_ptr(), _is_f32(table), max(table.stride(0), d), table.shape[0], d,
-                                            scale, out.data_ptr(), max(out.stride(0), d), self._stream()), "of_embedding_fwd")
+        n, (vocab, d) = ids.numel(), table.shape
+        assert ids.dtype is torch.int64 and ids.dim() == 1 and ids.is_contiguous() and out.dtype is table.dtype and out.shape == (n, d)
+        (ldt, ct), (ldy, cy) = table.stride(), out.stride()
+        assert ct == 1 and cy == 1
+        rc = self.lib.of_embedding_fwd(ids.data_ptr(), n, table.data_ptr(), _is_f32(table), max(ldt, d), vocab, d, scale, out.data_ptr(), max(ldy, d),
+                                       self._stream_fn())
+        if rc:
+            self._chk(rc, "of_embedding_fwd")
 
     def embedding_bwd(self, ids, dy, dw, scale=1.0, padding_idx=-1):
         """dw[v] = scale * sum of dy[i] over ids[i] == v, every row written; positions with padding_idx or an id outside dw add nothing."""

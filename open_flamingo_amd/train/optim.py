@@ -13,6 +13,8 @@ cross-attention parameters (open_flamingo/train/train.py:392-408).  Differences,
   that group has no weight decay, so AdamW leaves every other row untouched (zero moments): updating just those rows is
   the dense update.
 """
+import contextlib
+
 import torch
 
 from ..hip import abi
@@ -424,40 +426,40 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=0, lr=1e-3, betas=(
     lrs, wds = (list(x) if isinstance(x, (list, tuple)) else [x] * n for x in (lr, weight_decay))
     if len(lrs) != n or len(wds) != n:
         raise ValueError(f"{len(lrs)} learning rates and {len(wds)} weight decays for {n} parameters")
-    # one pass over the tensors: checks and descriptions (host time of a call, ~2 us a tensor)
-    dev, state, block = params[0].get_device(), torch.float8_e4m3fn if coded else F32, abi.ADAMW_BLOCK
-    table, at = [], set()
-    for i in range(n):
-        p, g, m, v = params[i], grads[i], exp_avgs[i], exp_avg_sqs[i]
-        k, pp = p.numel(), p.data_ptr()
-        bf16 = g.dtype is BF16
-        if not (p.dtype is F32 and (bf16 or g.dtype is F32) and m.dtype is state and v.dtype is state and g.numel() == k and m.numel() == k and v.numel() == k
-                and p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()
-                and p.get_device() == dev and g.get_device() == dev and m.get_device() == dev and v.get_device() == dev):
-            raise ValueError(f"tensor {i}: parameter, gradient and states must be contiguous, of one size, on one device, fp32 (gradient: or bf16; states: {state}), got "
-                             + ", ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in (p, g, m, v)))
-        a = b = 0
-        if coded:
-            ms, vs = exp_avg_scales[i], exp_avg_sq_scales[i]
-            if not (ms.dtype is F32 and vs.dtype is F32 and ms.is_contiguous() and vs.is_contiguous() and ms.numel() == vs.numel() == -(-k // block)
-                    and ms.get_device() == dev and vs.get_device() == dev):
-                raise ValueError(f"tensor {i}: one fp32 scale per {block} elements ({-(-k // block)} here), got {ms.dtype} {ms.numel()} and {vs.dtype} {vs.numel()}")
-            a, b = ms.data_ptr(), vs.data_ptr()
-        if k:
-            if pp in at:
-                raise ValueError(f"parameter {i} is listed twice")
-            at.add(pp)
-            table += (pp, g.data_ptr(), m.data_ptr(), v.data_ptr(), a, b, k, lrs[i], wds[i], bf16)
+    # checks and descriptions, a property of all tensors at a time (host time of a call: about a microsecond a tensor)
+    T = torch.Tensor
+    block, sizes = abi.ADAMW_BLOCK, list(map(T.numel, params))
+    state = torch.float8_e4m3fn if coded else F32
+    for name, ts, dtypes in (("parameter", params, {F32}), ("gradient", grads, {F32, BF16}), ("first moment", exp_avgs, {state}), ("second moment", exp_avg_sqs, {state})):
+        if not ({t.dtype for t in ts} <= dtypes and list(map(T.numel, ts)) == sizes and all(map(T.is_contiguous, ts))):
+            i = next(i for i, t in enumerate(ts) if t.dtype not in dtypes or t.numel() != sizes[i] or not t.is_contiguous())
+            raise ValueError(f"{name} {i} must be contiguous, {' or '.join(map(str, dtypes))}, of {sizes[i]} elements; got {ts[i].dtype} {tuple(ts[i].shape)} with strides {ts[i].stride()}")
+    every = [params, grads, exp_avgs, exp_avg_sqs]
+    if coded:
+        blocks = [-(-k // block) for k in sizes]
+        for name, ts in (("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales)):
+            if not ({t.dtype for t in ts} == {F32} and list(map(T.numel, ts)) == blocks and all(map(T.is_contiguous, ts))):
+                raise ValueError(f"{name}: one fp32 scale per {block} elements of a tensor, {blocks} here; got {[(t.dtype, t.numel()) for t in ts]}")
+        every += [exp_avg_scales, exp_avg_sq_scales]
+    dev = params[0].get_device()
+    if {d for ts in every for d in map(T.get_device, ts)} != {dev}:
+        raise ValueError(f"all tensors must be on one device, got {sorted({str(t.device) for ts in every for t in ts})}")
+    at = [list(map(T.data_ptr, ts)) for ts in every]
+    if not coded:
+        at += [[0] * n] * 2
+    table = [v for row in zip(*at, sizes, lrs, wds, [g.dtype is BF16 for g in grads]) if row[6] for v in row]
+    if len({p for p, k in zip(at[0], sizes) if k}) != sum(map(bool, sizes)):
+        raise ValueError("a parameter is listed twice")
     device = params[0].device
     if applied is not None and (applied.dtype != torch.int32 or applied.numel() != 1 or applied.device != device):
         raise ValueError("applied: one int32 on the parameters' device")
     if ops is None:
         _require_hip(params[0], "adamw_step")
         ops = Ops.default()
-    with torch.no_grad(), torch.cuda.device_of(params[0]):
-        sumsq = torch.empty(1, dtype=F32, device=device)
-        if not table:
-            return sumsq.zero_()
+    sumsq = torch.empty(1, dtype=F32, device=device)
+    if not table:
+        return sumsq.zero_()
+    with torch.cuda.device(dev) if dev >= 0 and dev != torch.cuda.current_device() else contextlib.nullcontext():
         ops.adamw_multi(table, sumsq, bits=8 if coded else 32, betas=betas, eps=eps, max_norm=max_norm, step=step, applied=applied)
     torch.autograd.graph.increment_version([*params, *exp_avgs, *exp_avg_sqs, *(exp_avg_scales or ()), *(exp_avg_sq_scales or ())])          # written behind autograd's back
     return sumsq

@@ -6,6 +6,7 @@ through them.  They stand beside ``towers.use_libofhip_lm_loss``, which computes
 ``sparse_rows``, which trains two rows of a frozen table.  GPU tensors only, like everything that runs on libofhip.
 """
 import types
+from contextlib import nullcontext
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -26,19 +27,30 @@ def _rows16(t):
     return t.contiguous() if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+def _on(t):
+    """Context in which libofhip launches on ``t``'s device (nothing to do where it is the current one)."""
+    at = t.get_device()
+    return nullcontext() if at < 0 or at == torch.cuda.current_device() else torch.cuda.device(at)
+
+
+def _linear_ce(hidden, table, labels, kw, ops, grad):
+    """(loss, what a backward needs)"""
+    x, w = _rows16(hidden), _rows16(table)
+    rows, d = x.shape
+    loss_rows = torch.empty(rows, dtype=F32, device=x.device)
+    loss = torch.empty((), dtype=F32, device=x.device) if kw["reduction"] != abi.CE_NONE else None
+    state = ops.linear_ce_state(rows, d, x.device, grad)
+    ops.linear_ce_fwd(x, w, labels, state, loss_rows, loss, **kw)
+    return loss_rows if loss is None else loss, (x, w, labels, state)
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, table, labels, ignore_index, reduction, logit_scale, piece, ops):
-        x, w = _rows16(hidden), _rows16(table)
-        rows, d = x.shape
-        loss_rows = torch.empty(rows, dtype=F32, device=x.device)
-        loss = torch.empty((), dtype=F32, device=x.device) if reduction != abi.CE_NONE else None
-        state = ops.linear_ce_state(rows, d, x.device)
-        kw = dict(ignore_index=ignore_index, logit_scale=logit_scale, reduction=reduction)
-        ops.linear_ce_fwd(x, w, labels, state, loss_rows, loss, **kw)
-        ctx.save_for_backward(x, w, labels, state)
-        ctx.kw, ctx.ops = dict(kw, piece=piece), ops
-        return loss_rows if loss is None else loss
+    def forward(ctx, hidden, table, labels, kw, piece, ops):
+        loss, saved = _linear_ce(hidden, table, labels, kw, ops, True)
+        ctx.save_for_backward(*saved)
+        ctx.kw, ctx.piece, ctx.ops = kw, piece, ops
+        return loss
 
     @staticmethod
     @once_differentiable
@@ -47,9 +59,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         need_x, need_w = ctx.needs_input_grad[:2]
         dx = torch.empty(x.shape, dtype=BF16, device=x.device) if need_x else None
         dw = torch.empty(w.shape, dtype=BF16, device=w.device) if need_w else None
-        with torch.cuda.device_of(x):
-            ctx.ops.linear_ce_bwd(x, w, labels, state, g.to(F32).contiguous(), dx, dw, **ctx.kw)
-        return dx, dw, None, None, None, None, None, None
+        with _on(x):
+            ctx.ops.linear_ce_bwd(x, w, labels, state, g.to(F32).contiguous(), dx, dw, piece=ctx.piece, **ctx.kw)
+        return dx, dw, None, None, None, None
 
 
 def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction="mean", logit_scale=1.0, piece=0, ops=None):
@@ -73,7 +85,7 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
         raise TypeError(f"labels must be int64, got {labels.dtype}")
     if piece < 0:
         raise ValueError("piece must not be negative")
-    if len({hidden.device, table.device, labels.device}) != 1:
+    if not hidden.get_device() == table.get_device() == labels.get_device():
         raise ValueError(f"hidden, table and labels are on {hidden.device}, {table.device} and {labels.device}")
     ops = _ops_for(hidden, ops, "linear_cross_entropy")
     dev = hidden.device.type
@@ -85,8 +97,12 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
     if x.shape[0] == 0:          # no rows: torch's values, zero gradients
         zero = (hidden.sum() + table[:0].sum()).to(F32)
         return zero.new_zeros(labels.shape) if reduction == "none" else zero / 0.0 if reduction == "mean" else zero
-    with torch.autocast(dev, enabled=False), torch.cuda.device_of(x):
-        out = _LinearCrossEntropy.apply(x, table, y, int(ignore_index), _REDUCTION[reduction], float(logit_scale), int(piece), ops)
+    kw = dict(ignore_index=int(ignore_index), logit_scale=float(logit_scale), reduction=_REDUCTION[reduction])
+    with _on(x):
+        if torch.is_grad_enabled() and (x.requires_grad or table.requires_grad):
+            out = _LinearCrossEntropy.apply(x, table, y, kw, int(piece), ops)
+        else:
+            out = _linear_ce(x, table, y, kw, ops, False)[0]
     return out.view(labels.shape) if reduction == "none" else out
 
 
@@ -106,7 +122,7 @@ class _EmbeddingLookup(torch.autograd.Function):
         if g.stride(-1) != 1:
             g = g.contiguous()
         dw = torch.empty(ctx.shape, dtype=g.dtype, device=g.device)
-        with torch.cuda.device_of(g):
+        with _on(g):
             ctx.ops.embedding_bwd(ids, g, dw, ctx.scale, ctx.padding_idx)
         return None, dw, None, None, None
 
@@ -117,25 +133,33 @@ def embedding_lookup(ids, table, *, scale=1.0, padding_idx=None, ops=None):
 
     ids: int64 of any shape; an id outside the table gives a row of NaN and no gradient.  padding_idx (None: none; negative: counted
     from the table's end): that row gets no gradient."""
-    if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
+    if table.dim() != 2 or 0 in table.shape:
         raise ValueError(f"table must be (vocabulary, d), got {tuple(table.shape)}")
-    if ids.dtype != torch.int64:
+    vocab, d = table.shape
+    if ids.dtype is not torch.int64:
         raise TypeError(f"ids must be int64, got {ids.dtype}")
-    if table.dtype not in (F32, BF16):
+    if table.dtype is not F32 and table.dtype is not BF16:
         raise TypeError(f"the table must be float32 or bfloat16, got {table.dtype}")
-    if ids.device != table.device:
+    if ids.get_device() != table.get_device():
         raise ValueError(f"ids and table are on {ids.device} and {table.device}")
     if padding_idx is not None:
-        if not -table.shape[0] <= padding_idx < table.shape[0]:
-            raise ValueError(f"padding_idx {padding_idx} is outside a table of {table.shape[0]} rows")
-        padding_idx %= table.shape[0]
-    ops = _ops_for(table, ops, "embedding_lookup")
-    if ids.numel() == 0:
-        return table[:0].reshape(*ids.shape, table.shape[1]) * scale
-    t = table if table.stride(1) == 1 and table.stride(0) >= table.shape[1] else table.contiguous()
-    with torch.cuda.device_of(t):
-        out = _EmbeddingLookup.apply(ids.reshape(-1).contiguous(), t, float(scale), -1 if padding_idx is None else padding_idx, ops)
-    return out.view(*ids.shape, table.shape[1])
+        if not -vocab <= padding_idx < vocab:
+            raise ValueError(f"padding_idx {padding_idx} is outside a table of {vocab} rows")
+        padding_idx %= vocab
+    if ops is None:
+        ops = _ops_for(table, ops, "embedding_lookup")
+    flat = ids if ids.dim() == 1 and ids.is_contiguous() else ids.reshape(-1).contiguous()
+    n = flat.shape[0]
+    if n == 0:
+        return table[:0].reshape(*ids.shape, d) * scale
+    t = table if table.stride(1) == 1 and table.stride(0) >= d else table.contiguous()
+    with _on(t):
+        if t.requires_grad and torch.is_grad_enabled():
+            out = _EmbeddingLookup.apply(flat, t, float(scale), -1 if padding_idx is None else padding_idx, ops)
+        else:
+            out = t.new_empty((n, d))
+            ops.embedding_fwd(flat, t, out, scale)
+    return out if ids.dim() == 1 else out.view(*ids.shape, d)
 
 
 def _ops_for(t, ops, what):

@@ -27,6 +27,14 @@ def test_loss_and_gradients(rows, d, vocab, piece, reduction, drop, scale):
     R.ce_check(lambda x, w, y, up: run(x, w, y, up, reduction, piece, scale), rows, d, vocab, reduction, drop, scale)
 
 
+@pytest.mark.parametrize("rows,d,vocab,reduction,drop", [(1, 8, 1, "mean", 0.0), (2, 72, 9, "none", 0.0), (3, 520, 50, "sum", 0.5), (8, 64, 2051, "mean", 0.4),
+                                                          (16, 136, 33, "none", 0.3), (9, 24, 7, "mean", 1.1)])
+def test_a_handful_of_rows_without_a_gradient(rows, d, vocab, reduction, drop):
+    def no_grad(x, w, y, up):
+        return linear_cross_entropy(x, w, y, reduction=reduction, ops=harness.emu_ops()), None, None
+    R.ce_check(no_grad, rows, d, vocab, reduction, drop)
+
+
 def test_strided_operands_and_labels_outside_the_vocabulary():
     x, w, y = R.ce_inputs(9, 64, 40, drop=0.2)
     y[4] = 2
@@ -42,6 +50,8 @@ def test_strided_operands_and_labels_outside_the_vocabulary():
     loss, gx, gw = run(x, w, bad, torch.ones(9), "none")
     assert torch.isnan(loss[4]) and torch.isfinite(loss[torch.arange(9) != 4]).all()
     assert (gx[4] == 0).all() and torch.isfinite(gw.float()).all()
+    few = linear_cross_entropy(x, w, bad, reduction="none", ops=harness.emu_ops())
+    assert torch.isnan(few[4]) and torch.allclose(few, loss, equal_nan=True)
     none = linear_cross_entropy(x[:0], w, y[:0], reduction="none", ops=harness.emu_ops())
     assert none.shape == (0,) and torch.isnan(linear_cross_entropy(x[:0], w, y[:0], ops=harness.emu_ops()))
 

@@ -34,6 +34,13 @@ def test_loss_and_gradients(rows, d, vocab, piece, reduction, drop, scale):
     R.ce_check(lambda x, w, y, up: run(x, w, y, up, reduction, piece, scale), rows, d, vocab, reduction, drop, scale, device=DEV)
 
 
+@pytest.mark.parametrize("rows,d,vocab,reduction", [(1, 2048, 50435, "none"), (2, 4096, 1003, "mean"), (4, 2560, 9001, "sum"), (7, 1024, 5000, "mean"),
+                                                     (16, 2048, 50435, "none"), (16, 2056, 3001, "mean"), (40, 512, 3001, "none")])
+def test_a_handful_of_rows_without_a_gradient(rows, d, vocab, reduction):
+    from open_flamingo_amd.train.vocab import linear_cross_entropy
+    R.ce_check(lambda x, w, y, up: (linear_cross_entropy(x, w, y, reduction=reduction), None, None), rows, d, vocab, reduction, 0.2, device=DEV)
+
+
 def test_no_gradient_and_one_gradient():
     x, w, y = R.ce_inputs(300, 512, 2000, device=DEV)
     both = run(x, w, y, torch.ones((), device=DEV))
