@@ -47,26 +47,34 @@ OF_GLOBAL void OF_BOUNDS(256, 4) emb_fwd_kernel(EmbArgs a) {
     const bool inside = id >= 0 && id < a.vocab;
     const float bad = __builtin_nanf("");          // an id outside the table: a caller's mistake, read nowhere, visible everywhere
     const size_t src = inside ? (size_t)id * a.ldt : 0, dst = (size_t)i * a.ldy;
-    if (a.vec && inside) {
-        const int vw = a.f32 ? 4 : 8;
-        if (a.f32) {
-            const float* t = (const float*)a.table + src;
-            float* o = (float*)a.y + dst;
-#pragma unroll 4
-            for (int c = lane * vw; c < a.d; c += 64 * vw) {
-                const f32x4 v = *(const f32x4*)(t + c);
-                *(f32x4*)(o + c) = f32x4{a.scale * v[0], a.scale * v[1], a.scale * v[2], a.scale * v[3]};
-            }
-        } else {
-            const bf16_t* t = (const bf16_t*)a.table + src;
-            bf16_t* o = (bf16_t*)a.y + dst;
-#pragma unroll 4
-            for (int c = lane * vw; c < a.d; c += 64 * vw) {
-                float x[8];
-                ofg::unpack8(*(const u32x4*)(t + c), x);
+    if (a.vec && inside) {          // eight 16-byte loads of a lane in flight
+        const int per = a.d / (a.f32 ? 4 : 8);
+        const u32x4* t = (const u32x4*)((const char*)a.table + src * (a.f32 ? 4 : 2));
+        u32x4* o = (u32x4*)((char*)a.y + dst * (a.f32 ? 4 : 2));
+        for (int c0 = 0; c0 < per; c0 += 512) {
+            u32x4 v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] *= a.scale;
-                *(u32x4*)(o + c) = ofg::pack8(x);
+            for (int u = 0; u < 8; ++u) {
+                const int c = c0 + u * 64 + lane;
+                if (c < per) v[u] = t[c];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int c = c0 + u * 64 + lane;
+                if (c >= per) break;
+                if (a.scale != 1.0f) {
+                    if (a.f32) {
+                        const f32x4 x = __builtin_bit_cast(f32x4, v[u]);
+                        v[u] = __builtin_bit_cast(u32x4, f32x4{a.scale * x[0], a.scale * x[1], a.scale * x[2], a.scale * x[3]});
+                    } else {
+                        float x[8];
+                        ofg::unpack8(v[u], x);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] *= a.scale;
+                        v[u] = ofg::pack8(x);
+                    }
+                }
+                o[c] = v[u];
             }
         }
         return;
@@ -282,13 +290,25 @@ template <bool F32, bool VEC>
 struct EmbVec {
     static constexpr int W = VEC ? (F32 ? 4 : 8) : 1;
 };
+// as it lies in memory (so that loads stay in flight), and added to a sum
 template <bool F32, bool VEC>
-OF_DEV void emb_load(const void* base, size_t at, float (&x)[8]) {
-    if constexpr (!VEC) x[0] = F32 ? ((const float*)base)[at] : of_bf16_to_f32(((const bf16_t*)base)[at]);
+OF_DEV u32x4 emb_raw(const void* base, size_t at) {
+    if constexpr (VEC) return *(const u32x4*)((const char*)base + at * (F32 ? 4 : 2));
+    else return u32x4{F32 ? ((const unsigned*)base)[at] : (unsigned)((const bf16_t*)base)[at], 0u, 0u, 0u};
+}
+template <bool F32, bool VEC>
+OF_DEV void emb_add(u32x4 v, float (&s)[8]) {
+    if constexpr (!VEC) s[0] += F32 ? __builtin_bit_cast(float, v[0]) : of_bf16_to_f32((bf16_t)v[0]);
     else if constexpr (F32) {
-        const f32x4 v = *(const f32x4*)((const float*)base + at);
-        x[0] = v[0]; x[1] = v[1]; x[2] = v[2]; x[3] = v[3];
-    } else ofg::unpack8(*(const u32x4*)((const bf16_t*)base + at), x);
+        const f32x4 x = __builtin_bit_cast(f32x4, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += x[e];
+    } else {
+        float x[8];
+        ofg::unpack8(v, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += x[e];
+    }
 }
 template <bool F32, bool VEC>
 OF_DEV void emb_store(void* base, size_t at, const float (&x)[8], float sc) {
@@ -306,21 +326,24 @@ OF_DEV void emb_store(void* base, size_t at, const float (&x)[8], float sc) {
 
 constexpr int AHEAD = 8;          // rows of dy in flight per thread
 
-// grid (chunks, column blocks).  part[chunk][0]: the sum of a token that began in an earlier chunk, [1]: of one that begins here and goes
-// on behind this chunk's end (a token that fills the whole chunk and does both counts as [0]).
+// grid (chunks, column blocks).  part[chunk][0]: the sum of a token that began in an earlier chunk, [1]: of one that begins here and
+// goes on behind this chunk's end (a token that fills the whole chunk and does both counts as [0]).  64 entries of the list at a time sit
+// in a register, one a lane: the walk reads them with v_readlane.
 template <bool F32, bool VEC>
 OF_GLOBAL void OF_BOUNDS(VEC_THREADS, 4) emb_sum_kernel(EmbArgs a) {
     typedef EmbVec<F32, VEC> V;
     const long chunk = of_bid_x(), lo = chunk * a.chunk, hi = lo + a.chunk < a.n ? lo + a.chunk : a.n;
+    const int lane = of_tid() & 63;
     const int col = (of_bid_y() * VEC_THREADS + of_tid()) * V::W;
-    if (col >= a.d) return;
+    const bool mine = col < a.d;
     const unsigned none = (unsigned)a.vocab;
+    const unsigned before = lo > 0 ? a.key[lo - 1] : none, behind = hi < a.n ? a.key[hi] : none;
     unsigned cur = a.key[lo];
-    bool head = lo > 0 && a.key[lo - 1] == cur;
+    bool head = lo > 0 && before == cur;
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    auto flush = [&](bool behind) OF_INLINE_LAMBDA {      // behind: the token goes on in the next chunk
-        if (cur == none) return;
-        if (head || behind) {
+    auto flush = [&](bool goes_on) OF_INLINE_LAMBDA {
+        if (cur == none || !mine) return;
+        if (head || goes_on) {
             float* p = a.part + ((size_t)chunk * 2 + (head ? 0 : 1)) * a.d + col;
 #pragma unroll
             for (int e = 0; e < V::W; ++e) p[e] = s[e];
@@ -328,32 +351,40 @@ OF_GLOBAL void OF_BOUNDS(VEC_THREADS, 4) emb_sum_kernel(EmbArgs a) {
             emb_store<F32, VEC>(a.dw, (size_t)cur * a.lddw + col, s, a.scale);
         }
     };
-    for (long i = lo; i < hi; i += AHEAD) {
-        if (a.key[i] == none) break;          // sorted: nothing but positions without a gradient from here on
-        float x[AHEAD][8];
+    for (long i0 = lo; i0 < hi; i0 += 64) {
+        const int len = hi - i0 < 64 ? (int)(hi - i0) : 64;
+        const long at = i0 + (lane < len ? lane : len - 1);
+        const unsigned key = a.key[at], pos = a.pos[at];
+        for (int i = 0; i < len; i += AHEAD) {
+            if (of_readlane(key, i) == none) break;          // sorted: nothing but positions without a gradient from here on
+            u32x4 x[AHEAD];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const long at = i + u < hi ? i + u : hi - 1;
-            emb_load<F32, VEC>(a.dy, (size_t)a.pos[at] * a.lddy + col, x[u]);
-        }
+            for (int u = 0; u < AHEAD; ++u) {
+                const size_t row = of_readlane(pos, i + u < len ? i + u : len - 1);
+                x[u] = emb_raw<F32, VEC>(a.dy, row * a.lddy + (mine ? col : 0));
+            }
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            if (i + u < hi) {
-                const unsigned k = a.key[i + u];
-                if (k != cur) {
-                    flush(false);
-                    cur = k;
-                    head = false;
+            for (int u = 0; u < AHEAD; ++u) {
+                const unsigned k = of_readlane(key, i + u < len ? i + u : len - 1);
+                if (i + u < len) {
+                    if (k != cur) {
+                        flush(false);
+                        cur = k;
+                        head = false;
 #pragma unroll
-                    for (int e = 0; e < V::W; ++e) s[e] = 0.f;
+                        for (int e = 0; e < V::W; ++e) s[e] = 0.f;
+                    }
+                    emb_add<F32, VEC>(x[u], s);
                 }
-#pragma unroll
-                for (int e = 0; e < V::W; ++e) s[e] += x[u][e];
             }
         }
+        if (of_readlane(key, len - 1) == none && cur != none) {          // the last token of the list ended in these 64
+            flush(false);
+            cur = none;
+        }
+        if (cur == none) return;
     }
-    if (a.key[hi - 1] != none) flush(hi < a.n && a.key[hi] == cur);
-    else if (cur != none) flush(false);
+    flush(behind == cur);
 }
 
 // grid (chunks, column blocks): the chunk whose last token begins there and goes on adds what the following chunks hold of it

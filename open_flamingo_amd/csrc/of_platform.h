@@ -362,6 +362,7 @@ OF_DEV float of_exp(float x) { return __expf(x); }
 // bare v_exp_f32 / v_log_f32 (base 2, no denormal fix-up sequence): softmax in the log2 domain
 OF_DEV float of_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 OF_DEV float of_log2(float x) { return __builtin_amdgcn_logf(x); }
+OF_DEV float of_min(float a, float b) { return __builtin_fminf(a, b); }
 OF_DEV float of_max(float a, float b) { return __builtin_fmaxf(a, b); }      // v_max_f32 (a ?: b keeps NaN order: cmp + cndmask)
 // Reductions over the four 16-lane rows of a wave (lanes l, l^16, l^32, l^48) without the LDS round trips of
 // ds_bpermute: v_permlane16_swap / v_permlane32_swap (gfx950) exchange rows between two registers inside the VALU.
@@ -408,6 +409,10 @@ OF_DEV unsigned of_f32_to_fp8x4(f32x4 v) {
 OF_DEV bool of_wave_any(bool p) { return __builtin_amdgcn_ballot_w64(p) != 0; }
 // 1-ulp hardware reciprocal (v_rcp_f32) instead of the ~12-instruction IEEE division sequence
 OF_DEV float of_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+// 1-ulp hardware square root (v_sqrt_f32; values below the normal range count as zero)
+OF_DEV float of_sqrt(float x) { return __builtin_amdgcn_sqrtf(x); }
+// the value of lane `src` (wave-uniform) in a scalar register
+OF_DEV unsigned of_readlane(unsigned v, int src) { return (unsigned)__builtin_amdgcn_readlane((int)v, src); }
 typedef __bf16 of_bf16x2n __attribute__((ext_vector_type(2)));
 // c + a.lo*b.lo + a.hi*b.hi on packed bf16 pairs, fp32 accumulate, ONE v_dot2c_f32_bf16 (gfx950)
 OF_DEV float of_dot2_bf16(unsigned a, unsigned b, float c) {

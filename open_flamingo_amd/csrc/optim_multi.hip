@@ -40,10 +40,18 @@ struct MtArgs {
     int chunk_end[MT_MAX];                  // cumulative chunks
     float beta1, omb1, beta2, omb2, eps;
     MtStep* step;
-    float* parts;
     MtTensor t[MT_MAX];
 };
-static_assert(sizeof(MtArgs) <= 4096, "kernel arguments");
+constexpr int MT_NORM_CHUNK = 8192;
+constexpr int MT_NORM_MAX = 196;            // the norm needs less of a tensor: more of them per launch
+struct MtNormArgs {
+    int n;
+    int chunk_end[MT_NORM_MAX];
+    float* parts;
+    unsigned long long g[MT_NORM_MAX];      // address, plus 1 for bf16
+    long count[MT_NORM_MAX];
+};
+static_assert(sizeof(MtArgs) <= 4096 && sizeof(MtNormArgs) <= 4096, "kernel arguments");
 struct MtBeginArgs {
     const float* parts; long count;
     float max_norm; double beta1, beta2;
@@ -106,21 +114,30 @@ OF_DEV void mt_store_codes(void* base, bool vec, long i, long n, unsigned u) {
 }
 
 // ------------------------------------------------------------------------------------------------ the norm
-// workgroup b of MT_PARTS sums the squares of chunks b, b + MT_PARTS, ...: the slot -> element assignment depends on the sizes alone
-OF_GLOBAL void OF_BOUNDS(256, 4) mt_sumsq_kernel(MtArgs a) {
+// Workgroup b of MT_PARTS takes chunks b, b + MT_PARTS, ... (32 KB each: the grid as a whole walks memory front to back -- with a long run of
+// its own for every workgroup the same pass read 3.6 TB/s); which slot sums which elements depends on the sizes alone
+OF_GLOBAL void OF_BOUNDS(256, 4) mt_sumsq_kernel(MtNormArgs a) {
     float* red = (float*)of_smem();
     const int tid = of_tid(), all = a.chunk_end[a.n - 1];
-    float s = 0.f;
+    int k = 0;
+    float s = 0.f, s2 = 0.f;
     for (int c = of_bid_x(); c < all; c += MT_PARTS) {
-        int first;
-        const MtTensor& t = a.t[mt_find(a, c, first)];
-        const long base = (long)(c - first) * MT_CHUNK + tid * 4;
-        f32x4 g[4];
+        while (a.chunk_end[k] <= c) ++k;
+        const unsigned long long at = a.g[k];
+        const int bf16 = (int)(at & 1);          // (gradients are at even addresses: the lowest bit tells the type)
+        const void* g0 = (const void*)(at & ~1ull);
+        const bool vec = !(at & (bf16 ? 6 : 14));
+        const long i = (long)(c - (k ? a.chunk_end[k - 1] : 0)) * MT_NORM_CHUNK + tid * 4, n = a.count[k];
+        f32x4 g[8];          // eight loads of a lane in flight
 #pragma unroll
-        for (int u = 0; u < 4; ++u) g[u] = mt_load(t.g, t.flags & 1, t.flags & 2, base + u * 1024, t.n);
+        for (int u = 0; u < 8; ++u) g[u] = mt_load(g0, bf16, vec, i + u * 1024, n);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) s += (g[u][0] * g[u][0] + g[u][1] * g[u][1]) + (g[u][2] * g[u][2] + g[u][3] * g[u][3]);
+        for (int u = 0; u < 8; u += 2) {
+            s += (g[u][0] * g[u][0] + g[u][1] * g[u][1]) + (g[u][2] * g[u][2] + g[u][3] * g[u][3]);
+            s2 += (g[u + 1][0] * g[u + 1][0] + g[u + 1][1] * g[u + 1][1]) + (g[u + 1][2] * g[u + 1][2] + g[u + 1][3] * g[u + 1][3]);
+        }
     }
+    s += s2;
     s = of_wave_sum(s);
     if ((tid & 63) == 0) red[tid >> 6] = s;
     of_sync();
@@ -166,28 +183,26 @@ OF_DEV unsigned mt_random20(unsigned key, long i) {
 // q in [0, 448] to a neighbouring e4m3 value, the upper one with the probability of q's place between the two (u: 20 random bits);
 // above zero stays above zero
 OF_DEV float mt_round_random(float q, unsigned u) {
-    if (!(q > 0.f)) return 0.f;
-    float r;
-    if (q >= 0.015625f) {                   // 2^-6, the smallest normal value: 20 of the 23 mantissa bits go
-        r = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, q) + u) & 0xFFF00000u);
-        r = r < 448.0f ? r : 448.0f;
-    } else {                                // below, values are 2^-9 apart
-        r = floorf(q * 512.0f + (float)u * 0x1p-20f) * (1.0f / 512.0f);
-        r = r > (1.0f / 512.0f) ? r : 1.0f / 512.0f;
-    }
-    return r;
+    // from 2^-6, the smallest normal value, 20 of the 23 mantissa bits go; below, values are 2^-9 apart
+    const float n = of_min(__builtin_bit_cast(float, (__builtin_bit_cast(unsigned, q) + u) & 0xFFF00000u), 448.0f);
+    const float d = of_max(floorf(q * 512.0f + (float)u * 0x1p-20f) * (1.0f / 512.0f), 1.0f / 512.0f);
+    return q >= 0.015625f ? n : q > 0.f ? d : 0.f;
 }
 
 struct MtHyper {
     float coef, step_size, inv_sqrt_bc2, decay, beta1, omb1, beta2, omb2, eps;
 };
-OF_DEV void mt_update(const MtHyper& h, f32x4& p, f32x4 g, f32x4& m, f32x4& v) {
+// r receives the square root of the second moment
+OF_DEV void mt_update(const MtHyper& h, f32x4& p, f32x4 g, f32x4& m, f32x4& v, f32x4& r) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const float ge = h.coef * g[e];
         m[e] = h.beta1 * m[e] + h.omb1 * ge;
         v[e] = h.beta2 * v[e] + h.omb2 * ge * ge;
-        p[e] = h.decay * p[e] - h.step_size * (m[e] / (sqrtf(v[e]) * h.inv_sqrt_bc2 + h.eps));
+        // 1-ulp reciprocal and square root: 2e-7 of an update that is itself a thousandth of the parameter (the IEEE forms are ~25
+        // instructions an element more, and 8-bit states are bound by instructions, not by memory)
+        r[e] = of_sqrt(v[e]);
+        p[e] = h.decay * p[e] - h.step_size * (m[e] * of_rcp(r[e] * h.inv_sqrt_bc2 + h.eps));
     }
 }
 
@@ -225,7 +240,8 @@ OF_GLOBAL void OF_BOUNDS(256, 4) mt_adamw_kernel(MtArgs a) {
     for (int u = 0; u < 4; ++u) {
         const long i = base + u * BLOCK;
         if (BITS == 32) {
-            mt_update(h, p[u], g[u], m[u], v[u]);
+            f32x4 r;
+            mt_update(h, p[u], g[u], m[u], v[u], r);
             mt_store(t.p, vec, i, n, p[u]);
             mt_store((float*)t.m, vec, i, n, m[u]);
             mt_store((float*)t.v, vec, i, n, v[u]);
@@ -239,27 +255,29 @@ OF_GLOBAL void OF_BOUNDS(256, 4) mt_adamw_kernel(MtArgs a) {
                 v[u][e] *= vs[u];
                 v[u][e] *= v[u][e];
             }
-            mt_update(h, p[u], g[u], m[u], v[u]);
+            f32x4 r;
+            mt_update(h, p[u], g[u], m[u], v[u], r);
             mt_store(t.p, vec, i, n, p[u]);
+            if (i + 4 > n) {          // behind the tensor's end: zeros, which no block's largest is
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + e >= n) m[u][e] = r[e] = 0.f;
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v[u][e] = sqrtf(v[u][e]);
-                if (i + e >= n) m[u][e] = v[u][e] = 0.f;
-                tm = of_max(tm, fabsf(m[u][e]));
-                tr = of_max(tr, v[u][e]);
+                tm = of_max(tm, __builtin_fabsf(m[u][e]));
+                tr = of_max(tr, r[e]);
             }
             tm = of_wave_max(tm);
             tr = of_wave_max(tr);
-            const float im = 448.0f / of_max(tm, 1e-30f), ir = 448.0f / of_max(tr, 1e-30f);
+            const float im = 448.0f / of_max(tm, 1e-30f), ir = 448.0f / of_max(tr, 1e-30f);          // (IEEE: once a block)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float q = m[u][e] * im;
-                m[u][e] = q > 448.0f ? 448.0f : q < -448.0f ? -448.0f : q;
-                const float r = v[u][e] * ir;
-                v[u][e] = mt_round_random(r > 448.0f ? 448.0f : r, mt_random20(key, i + e));
+                m[u][e] = of_max(of_min(m[u][e] * im, 448.0f), -448.0f);
+                r[e] = mt_round_random(of_min(r[e] * ir, 448.0f), mt_random20(key, i + e));
             }
             mt_store_codes(t.m, vec, i, n, of_f32_to_fp8x4(m[u]));
-            mt_store_codes(t.v, vec, i, n, of_f32_to_fp8x4(v[u]));
+            mt_store_codes(t.v, vec, i, n, of_f32_to_fp8x4(r));
             if (lane == 0 && i < n) {
                 t.ms[i / BLOCK] = tm / 448.0f;
                 t.vs[i / BLOCK] = tr / 448.0f;
@@ -268,11 +286,11 @@ OF_GLOBAL void OF_BOUNDS(256, 4) mt_adamw_kernel(MtArgs a) {
     }
 }
 
-int mt_launches(int n) { return (n + MT_MAX - 1) / MT_MAX; }
+int mt_launches(int n, int per) { return (n + per - 1) / per; }
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 }  // namespace
 
-extern "C" size_t of_adamw_multi_workspace_bytes(int n) { return n > 0 ? up256(sizeof(MtStep)) + (size_t)mt_launches(n) * MT_PARTS * sizeof(float) : 0; }
+extern "C" size_t of_adamw_multi_workspace_bytes(int n) { return n > 0 ? up256(sizeof(MtStep)) + (size_t)mt_launches(n, MT_NORM_MAX) * MT_PARTS * sizeof(float) : 0; }
 
 extern "C" int of_adamw_multi(const OfAdamwTensor* tensors, int n, int bits, double beta1, double beta2, double eps, double max_norm, int step, int* applied_steps,
                               float* sumsq, void* workspace, size_t workspace_bytes, void* stream) {
@@ -290,7 +308,8 @@ extern "C" int of_adamw_multi(const OfAdamwTensor* tensors, int n, int bits, dou
     of_stream_t s = (of_stream_t)stream;
     MtStep* st = (MtStep*)workspace;
     float* parts = (float*)((char*)workspace + up256(sizeof(MtStep)));
-    const int launches = mt_launches(n);
+    const int launches = mt_launches(n, MT_MAX), norms = mt_launches(n, MT_NORM_MAX);
+    auto chunks = [](long elements, int chunk) { return (elements + chunk - 1) / chunk; };
     auto pack = [&](int l, MtArgs& a) {
         a = MtArgs{};
         long end = 0;
@@ -302,25 +321,39 @@ extern "C" int of_adamw_multi(const OfAdamwTensor* tensors, int n, int bits, dou
             const uintptr_t state = (uintptr_t)t.m | (uintptr_t)t.v;
             d.flags = (t.g_bf16 ? 1 : 0) | (!(wide & 15) && !(state & (bits == 32 ? 15 : 3)) ? 2 : 0);
             d.ordinal = i;
-            end += (t.n + MT_CHUNK - 1) / MT_CHUNK;
+            end += chunks(t.n, MT_CHUNK);
             a.chunk_end[a.n++] = (int)end;
         }
         a.beta1 = (float)beta1; a.omb1 = (float)(1.0 - beta1); a.beta2 = (float)beta2; a.omb2 = (float)(1.0 - beta2); a.eps = (float)eps;
         a.step = st;
-        a.parts = parts + (size_t)l * MT_PARTS;
         return end;
     };
-    MtArgs a;
-    for (int l = 0; l < launches; ++l)
-        if (pack(l, a) >= 1l << 31) return OF_E_SHAPE;
-    for (int l = 0; l < launches; ++l) {
-        pack(l, a);
-        const int rc = of_launch(mt_sumsq_kernel, of_dim3{MT_PARTS, 1, 1}, 256, 4 * sizeof(float), s, a);
-        if (rc) return rc;
+    long most = 0;
+    for (int l = 0; l < norms; ++l) {
+        long end = 0;
+        for (int i = l * MT_NORM_MAX; i < n && i < (l + 1) * MT_NORM_MAX; ++i) end += chunks(tensors[i].n, MT_CHUNK);
+        if (end > most) most = end;
     }
-    const MtBeginArgs b{parts, (long)launches * MT_PARTS, (float)max_norm, beta1, beta2, step, applied_steps, st, sumsq};
-    int rc = of_launch(mt_begin_kernel, of_dim3{1, 1, 1}, 256, 4 * sizeof(float), s, b);
-    for (int l = 0; l < launches && !rc; ++l) {
+    if (most >= 1l << 31) return OF_E_SHAPE;          // (the updates' launches hold fewer tensors)
+    int rc = 0;
+    for (int l = 0; l < norms && !rc; ++l) {
+        MtNormArgs a{};
+        long end = 0;
+        for (int i = l * MT_NORM_MAX; i < n && i < (l + 1) * MT_NORM_MAX; ++i) {
+            end += chunks(tensors[i].n, MT_NORM_CHUNK);
+            a.g[a.n] = (unsigned long long)(uintptr_t)tensors[i].g | (tensors[i].g_bf16 ? 1 : 0);
+            a.count[a.n] = tensors[i].n;
+            a.chunk_end[a.n++] = (int)end;
+        }
+        a.parts = parts + (size_t)l * MT_PARTS;
+        rc = of_launch(mt_sumsq_kernel, of_dim3{MT_PARTS, 1, 1}, 256, 4 * sizeof(float), s, a);
+    }
+    if (rc) return rc;
+    const MtBeginArgs b{parts, (long)norms * MT_PARTS, (float)max_norm, beta1, beta2, step, applied_steps, st, sumsq};
+    rc = of_launch(mt_begin_kernel, of_dim3{1, 1, 1}, 256, 4 * sizeof(float), s, b);
+    // last tensors first: the norm's launch read their gradients last, up to 256 MB of them are still in the Infinity Cache
+    for (int l = launches - 1; l >= 0 && !rc; --l) {
+        MtArgs a;
         const unsigned grid = (unsigned)pack(l, a);
         rc = bits == 8 ? of_launch(mt_adamw_kernel<8>, of_dim3{grid, 1, 1}, 256, 0, s, a) : of_launch(mt_adamw_kernel<32>, of_dim3{grid, 1, 1}, 256, 0, s, a);
     }

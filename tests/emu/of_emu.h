@@ -305,6 +305,16 @@ OF_DEV float of_shfl(float v, int src) {
     of_emu::wave_barrier();
     return r;
 }
+OF_DEV float of_emu_float(unsigned u) {
+    float f;
+    memcpy(&f, &u, 4);
+    return f;
+}
+OF_DEV unsigned of_emu_bits(float f) {
+    unsigned u;
+    memcpy(&u, &f, 4);
+    return u;
+}
 OF_DEV float of_shfl_xor(float v, int m) { return of_shfl(v, (of_emu::g_blk->cur & 63) ^ m); }
 OF_DEV int of_shfl_xor_i(int v, int m) {
     float f;
@@ -368,6 +378,7 @@ OF_DEV float of_rows_sum(float x) {
 OF_DEV float of_exp2(float x) { return exp2f(x); }
 OF_DEV float of_log2(float x) { return log2f(x); }
 OF_DEV float of_max(float a, float b) { return fmaxf(a, b); }
+OF_DEV float of_min(float a, float b) { return fminf(a, b); }
 OF_DEV void of_atomic_add(float* p, float v) {
     std::atomic<unsigned>* a = (std::atomic<unsigned>*)p;
     unsigned old = a->load();
@@ -382,6 +393,8 @@ OF_DEV void of_atomic_add(float* p, float v) {
 }
 OF_DEV float of_exp(float x) { return expf(x); }
 OF_DEV float of_rcp(float x) { return 1.0f / x; }
+OF_DEV float of_sqrt(float x) { return sqrtf(x); }
+OF_DEV unsigned of_readlane(unsigned v, int src) { return (unsigned)of_emu_bits(of_shfl(of_emu_float(v), src)); }
 OF_DEV float of_erf(float x) { return erff(x); }
 OF_DEV float of_tanh(float x) { return tanhf(x); }
 OF_DEV float of_rsqrt(float x) { return 1.0f / sqrtf(x); }
