@@ -375,16 +375,18 @@ int of_ce_bwd(const void* logits, int logits_f32, long ld, const long long* labe
  *   x: rows x d bf16 (row stride ldx), w: vocab x d bf16 (row stride ldw), labels: rows int64, already shifted by the caller.
  *   of_linear_ce_fwd: loss_rows[row] as of_ce_fwd; *loss = their sum (OF_CE_SUM) or the sum / number of labels that count (OF_CE_MEAN: NaN
  *              without any); OF_CE_NONE writes loss_rows alone.  `state` receives what the backward needs (the rows whose label counts,
- *              gathered, and their log-sum-exp): of_linear_ce_state_bytes(rows, d) bytes, untouched by the caller in between.
+ *              gathered, and their log-sum-exp): of_linear_ce_state_bytes(args) bytes, untouched by the caller in between.
  *   of_linear_ce_bwd: dx (rows x d, row stride lddx) and / or dw (vocab x d, row stride lddw), both bf16, either may be NULL; *grad
  *              (OF_CE_NONE: grad[row]) is the upstream gradient, on the device.  Rows that are ignored, or whose label lies outside the
  *              vocabulary, get zeros and add nothing.  The same x, w, labels, rows, vocab, d, logit_scale and reduction as the forward.
  *              The vocabulary is walked in pieces of `piece` rows (rounded down to a multiple of 256, at least 256; 0: chosen so that a
  *              piece of the logits' gradient, rows x piece bf16, takes 128 MB).
+ *              early_dx = 1 (dx wanted, dw not: a frozen table; the same in forward and backward): the forward sums dx as well, in `state`, from
+ *              the one logits product, and the backward only finishes it.
  *              of_linear_ce_stateless(rows, d) = 1 (a handful of rows: scoring next tokens): `state` may be NULL, with no backward to follow
  * Deterministic: no atomics.  d % 8 == 0; x, w, dx, dw 16-byte aligned like state and workspace, row strides
- * multiples of 8.  The workspace holds of_linear_ce_workspace_bytes(args, backward) bytes: the fields rows, vocab, d, piece, reduction,
- * state and (backward) dx of args decide. */
+ * multiples of 8.  The workspace holds of_linear_ce_workspace_bytes(args, backward) bytes: the fields rows, vocab, d, ldw, piece, early_dx,
+ * reduction, state and (backward) dx of args decide. */
 enum { OF_CE_NONE = 0, OF_CE_MEAN = 1, OF_CE_SUM = 2 };
 typedef struct OfLinearCeArgs {
     const uint16_t* x; long ldx;
@@ -401,9 +403,10 @@ typedef struct OfLinearCeArgs {
     uint16_t* dx; long lddx;
     uint16_t* dw; long lddw;
     int piece;
+    int early_dx;
     void* workspace; size_t workspace_bytes;
 } OfLinearCeArgs;
-size_t of_linear_ce_state_bytes(long rows, int d);
+size_t of_linear_ce_state_bytes(const OfLinearCeArgs* args);      /* rows, vocab, d, ldw, piece and early_dx of args decide */
 int of_linear_ce_stateless(long rows, int d);
 size_t of_linear_ce_workspace_bytes(const OfLinearCeArgs* args, int backward);
 int of_linear_ce_fwd(const OfLinearCeArgs* args, void* stream);

@@ -6,6 +6,9 @@
 //   DLOGIT  the same product again: D = exp(z - lse[row]) - [column == label], times the row's upstream gradient where rows have one of
 //           their own, stored as bf16 (the operand type of the two products behind it; half a unit of 2^-8 of each entry at most).  A
 //           scalar upstream gradient is NOT in D -- it multiplies the fp32 sums of those products instead, so that -1 + p keeps its bits.
+//   EARLY   the product once for both, where the table's gradient is not wanted: E = exp(z - c[row]) as bf16, 0 at the label, and its fp32 sum
+//           per row and 128-column strip (the label's included) -> part[strip][row]; the label's z -> zlab[row].  c, the label's logit from a
+//           dot product of its own, is never above the log-sum-exp, and E overflows only where a row's loss is above 80 (linear_ce.hip)
 //   DX      dx_acc (fp32) = beta dx_acc + D W over the pieces of the vocabulary; with few tiles (few rows) the piece is split along the
 //           vocabulary into of_ce_splits parts, each with a dx_acc of its own
 //   DW      dW (bf16) = scale D^T x
@@ -14,7 +17,7 @@
 #pragma once
 #include "gemm_tile256.h"
 
-enum { OF_EPI_CE_LSE = 16, OF_EPI_CE_DLOGIT = 17, OF_EPI_CE_DX = 18, OF_EPI_CE_DW = 19 };      // internal: of_gemm refuses them
+enum { OF_EPI_CE_LSE = 16, OF_EPI_CE_DLOGIT = 17, OF_EPI_CE_DX = 18, OF_EPI_CE_DW = 19, OF_EPI_CE_EARLY = 20 };      // internal: of_gemm refuses them
 OF_HOSTDEV constexpr bool of_epi_is_ce(int epi) { return epi >= OF_EPI_CE_LSE; }
 
 struct OfCeGemmArgs : OfGemmArgs {      // M, N, K: the padded extents of the launch (of_gemm's layout rules)
@@ -22,12 +25,13 @@ struct OfCeGemmArgs : OfGemmArgs {      // M, N, K: the padded extents of the la
     long b_bytes;            // bytes of the B matrix from args.B to the end of its last row
     int n_valid;             // columns that exist (LSE, DLOGIT: vocabulary of the piece; DX, DW: d)
     int m_valid;             // DW: rows that exist (vocabulary of the piece)
-    int col0;                // vocabulary index of column 0 of the piece (labels count from the table's first row)
+    int col0;                // vocabulary index of column 0 of the piece (labels count from the table's first row; EARLY's strips too)
     const int* lab;          // [row] label, -1 for rows behind `count`
-    const float* lse;        // [row] in units of log 2, +inf for rows behind `count`
+    const int* gate;         // device flag or NULL: nothing is done where it is 0
+    const float* lse;        // [row] in units of log 2, +inf for rows behind `count` (EARLY: c)
     const float* grow;       // [row] upstream gradient of its own, or NULL
-    float* part;             // LSE: [strip][row][2]
-    float* zlab;             // LSE: [row]
+    float* part;             // LSE: [strip][row][2]; EARLY: [strip][row]
+    float* zlab;             // LSE, EARLY: [row]
     long part_ld;            // rows of one strip
     const float* gscale;     // DW: scalar upstream gradient or NULL (1)
     int by_count;            // DW: divide by `count`
@@ -39,6 +43,7 @@ template <int EPI>
 struct OfEpiArgs { typedef OfGemmArgs type; };
 template <> struct OfEpiArgs<OF_EPI_CE_LSE> { typedef OfCeGemmArgs type; };
 template <> struct OfEpiArgs<OF_EPI_CE_DLOGIT> { typedef OfCeGemmArgs type; };
+template <> struct OfEpiArgs<OF_EPI_CE_EARLY> { typedef OfCeGemmArgs type; };
 template <> struct OfEpiArgs<OF_EPI_CE_DX> { typedef OfCeGemmArgs type; };
 template <> struct OfEpiArgs<OF_EPI_CE_DW> { typedef OfCeGemmArgs type; };
 
@@ -106,7 +111,7 @@ OF_DEV void ce_lse_rows(const OfCeGemmArgs& p, Frag frag, int m_base, int n_base
 
 // the row passes of one 32 x 64 group (accumulators in the patch)
 template <int EPI>
-OF_DEV void ce_group_rows(const OfCeGemmArgs& p, char* patch, int m_base, int n_base, int lane, float sc) {
+OF_DEV void ce_group_rows(const OfCeGemmArgs& p, char* patch, int m_base, int n_base, int lane, float sc, float (&sum)[4]) {
     constexpr bool SPLIT = EPI == OF_EPI_CE_DX;          // fp32 output: columns 4j.. and 32 + 4j.. (gemm_common.h, epi_split_cols)
     const int hi = SPLIT ? 32 : 4;
     const int rd_row = lane >> 3, rd_col = (lane & 7) * (SPLIT ? 4 : 8);
@@ -116,7 +121,27 @@ OF_DEV void ce_group_rows(const OfCeGemmArgs& p, char* patch, int m_base, int n_
         const int r = it * 8 + rd_row, m = m_base + r, n = n_base + rd_col;
         const f32x4 v0 = *(const f32x4*)(patch + r * ofg::PATCH_PITCH + rd_col * 4), v1 = *(const f32x4*)(patch + r * ofg::PATCH_PITCH + (rd_col + hi) * 4);
         float a[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-        if constexpr (EPI == OF_EPI_CE_DLOGIT) {
+        if constexpr (EPI == OF_EPI_CE_EARLY) {
+            const int at = p.lab[m] - p.col0 - n;
+            const float c = p.lse[m];
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = of_exp2(__builtin_fmaf(a[e], sc, -c));
+            if (n_base + 64 > p.n_valid) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = n + e < p.n_valid ? o[e] : 0.f;
+            }
+            sum[it] += ((o[0] + o[1]) + (o[2] + o[3])) + ((o[4] + o[5]) + (o[6] + o[7]));
+            if ((unsigned)at < 8u) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e == at) {
+                        p.zlab[m] = a[e] * sc;
+                        o[e] = 0.f;
+                    }
+            }
+            *(u32x4*)((bf16_t*)p.C + (size_t)m * p.ldc + n) = ofg::pack8(o);
+        } else if constexpr (EPI == OF_EPI_CE_DLOGIT) {
             // what few elements need (the label's, columns behind the vocabulary) sits in branches
             const int at = p.lab[m] - p.col0 - n;         // the label's place among this lane's eight columns, if 0 <= at < 8
             const float l = p.lse[m];
@@ -176,12 +201,26 @@ template <int EPI, class ToPatch>
 OF_DEV void w4_epilogue_ce(const OfCeGemmArgs& p, ToPatch to_patch, char* smem, int m0, int n0, int wm, int wn, int wave, int lane) {
     char* patch = smem + wave * ofg::PATCH_BYTES;
     float sc = p.alpha;
-    if (EPI == OF_EPI_CE_DLOGIT) sc *= CE_LOG2E;
+    if (EPI == OF_EPI_CE_DLOGIT || EPI == OF_EPI_CE_EARLY) sc *= CE_LOG2E;
     if (EPI == OF_EPI_CE_DW) sc *= of_ce_scale(p.gscale, p.by_count, p.count);
+    float sum[4];
 #pragma unroll
     for (int g = 0; g < 8; ++g) {
+        if (!(g & 1)) sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
         to_patch(g, patch);
-        ce_group_rows<EPI>(p, patch, m0 + wm * 128 + (g >> 1) * 32, n0 + wn * 128 + (g & 1) * 64, lane, sc);
+        ce_group_rows<EPI>(p, patch, m0 + wm * 128 + (g >> 1) * 32, n0 + wn * 128 + (g & 1) * 64, lane, sc, sum);
+        if constexpr (EPI == OF_EPI_CE_EARLY) {
+            if (g & 1) {          // the strip's 128 columns of a row sit in eight lanes
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    float s = sum[it];
+#pragma unroll
+                    for (int o = 4; o >= 1; o >>= 1) s += of_shfl_xor(s, o);
+                    const int m = m0 + wm * 128 + (g >> 1) * 32 + it * 8 + (lane >> 3);
+                    if ((lane & 7) == 0) p.part[((size_t)((p.col0 + n0) >> 7) + wn) * p.part_ld + m] = s;
+                }
+            }
+        }
     }
 }
 

@@ -146,6 +146,7 @@ OF_GLOBAL void OF_BOUNDS(256, 1) of_gemm_w4m_kernel(typename OfEpiArgs<EPI>::typ
     static_assert(!CE || !SK, "classic launches only");
     int parts = 1;                        // DX: parts of K, each on a copy of C of its own
     if constexpr (CE) {
+        if (p.gate && of_uniform(*p.gate) == 0) return;
         const int live = of_ce_live_rows(of_uniform(*p.count));
         if (EPI == OF_EPI_CE_DW) p.K = live;
         else p.M = live;
@@ -528,6 +529,7 @@ int of_gemm_w4m_ce(const OfCeGemmArgs& a, of_stream_t s) {
     constexpr int smem = SMEM_W4M + OPER_BYTES;
     switch (a.epi) {
         case OF_EPI_CE_LSE: return of_launch(of_gemm_w4m_kernel<false, false, OF_EPI_CE_LSE, false>, grid, 256, smem, s, a);
+        case OF_EPI_CE_EARLY: return of_launch(of_gemm_w4m_kernel<false, false, OF_EPI_CE_EARLY, false>, grid, 256, smem, s, a);
         case OF_EPI_CE_DLOGIT: return of_launch(of_gemm_w4m_kernel<false, false, OF_EPI_CE_DLOGIT, false>, grid, 256, smem, s, a);
         case OF_EPI_CE_DX: return of_launch(of_gemm_w4m_kernel<false, true, OF_EPI_CE_DX, false>, grid, 256, smem, s, a);
         case OF_EPI_CE_DW: return of_launch(of_gemm_w4m_kernel<true, true, OF_EPI_CE_DW, false>, grid, 256, smem, s, a);

@@ -7,6 +7,9 @@
 //             keeps (max, sum exp) per row and 128 columns, from fp32 accumulators; a small launch joins the ~400 strips of a row;
 //   backward  the vocabulary in pieces: the product again -> D of the piece (bf16, at most a few hundred MB, sized so that it stays in
 //             the 256-MB Infinity Cache between the three products that touch it) -> dx += D W_piece in fp32, dW_piece = D^T x.
+//   frozen table   without dW the forward forms dx as well and the backward has no product left (two instead of three): E = exp(z - c) with
+//             c = the label's logit needs no maximum, dx = s g (exp(c - lse) E W + (p_label - 1) w_label).  lse - c is the row's loss; only a
+//             loss above 80 (in units of log 2) could overflow, and then a flag on the device lets the forms above run behind it.
 // All products run on the 256x256 MFMA kernel (gemm_w4m.hip) with the epilogues of gemm_ce_epi.h: they are bound by its K loop, i.e. by
 // the chip's power budget, 2 R V d operations forward and 6 R V d backward (a third of them the second logits product).
 // No atomics; every sum has a fixed order.
@@ -14,6 +17,7 @@
 
 namespace {
 
+constexpr float CE_FAR = 80.f;             // E <= 2^80: finite in bf16, and in fp32 sums of it
 constexpr int CE_THREADS = 512;          // of the launches that are one workgroup
 
 struct CeRowsArgs {
@@ -26,8 +30,23 @@ struct CeRowsArgs {
     float* loss; int mean;
     const float* grad; int by_count; float logit_scale; const float* acc; int split_stages; bf16_t* dx; long lddx;
     float* grow;
+    const int* gate;                           // device flag or NULL: nothing is done where it is 0
+    float* ref; int* far; float sc2;           // EARLY: c by place, "some loss is above CE_FAR", logit_scale * log2 e
     const bf16_t* w; long ldw; bf16_t* wc; long ldwc; long w_rows;
 };
+
+// EARLY's c: the label's logit in units of log 2, a dot product by the wave that gathers the row
+OF_DEV void ce_reference(const CeRowsArgs& a, const bf16_t* x, int lab, long i, int lane) {
+    const bf16_t* w = a.w + (size_t)lab * a.ldw;
+    float s = 0.f;
+    for (int c = lane * 8; c < a.d; c += 512) {
+        const u32x4 u = *(const u32x4*)(x + c), v = *(const u32x4*)(w + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = of_dot2_bf16(u[e], v[e], s);
+    }
+    s = of_wave_sum(s);
+    if (lane == 0) a.ref[i] = s * a.sc2;
+}
 
 // One workgroup: the rows whose label counts, in order.  slot_of[row] = place among them or -1, row_of its inverse, lab by place;
 // loss_rows of the others is final here: 0 for ignored rows, NaN for a label outside the vocabulary (a caller's mistake that has to
@@ -79,7 +98,10 @@ OF_GLOBAL void OF_BOUNDS(CE_THREADS, 1) ce_index_kernel(CeRowsArgs a) {
             }
         }
     }
-    if (tid == 0) *a.count = total;
+    if (tid == 0) {
+        *a.count = total;
+        if (a.far) *a.far = 0;
+    }
     for (int i = total + tid; i < of_ce_live_rows(total); i += CE_THREADS) a.lab[i] = -1;
 }
 
@@ -90,6 +112,10 @@ OF_GLOBAL void OF_BOUNDS(256, 4) ce_gather_kernel(CeRowsArgs a) {
     const long i = (long)of_bid_x() * 4 + (of_tid() >> 6);
     if (i >= of_ce_live_rows(count)) return;
     const bf16_t* src = i < count ? a.x + (size_t)a.row_of[i] * a.ldx : nullptr;
+    if (a.ref) {
+        if (src) ce_reference(a, src, a.lab[i], i, lane);
+        else if (lane == 0) a.ref[i] = 0.f;
+    }
     bf16_t* dst = a.xc + (size_t)i * a.ldxc;
     for (int c = lane * 8; c < a.d_pad; c += 512) {
         u32x4 v = {0u, 0u, 0u, 0u};
@@ -131,11 +157,18 @@ OF_GLOBAL void OF_BOUNDS(256, 4) ce_index_gather_kernel(CeRowsArgs a) {
     }
     const int live = of_ce_live_rows(at);
     if (of_bid_x() == 0 && wave == 0) {
-        if (lane == 0) *a.count = at;
+        if (lane == 0) {
+            *a.count = at;
+            if (a.far) *a.far = 0;
+        }
         for (int k = at + lane; k < live; k += 64) a.lab[k] = -1;
     }
     if (i >= live) return;
     const bf16_t* src = mine >= 0 ? a.x + (size_t)mine * a.ldx : nullptr;
+    if (a.ref) {
+        if (src) ce_reference(a, src, (int)a.labels[mine], i, lane);
+        else if (lane == 0) a.ref[i] = 0.f;
+    }
     bf16_t* dst = a.xc + (size_t)i * a.ldxc;
     for (int c = lane * 8; c < a.d_pad; c += 512) {
         u32x4 v = {0u, 0u, 0u, 0u};
@@ -159,10 +192,16 @@ OF_GLOBAL void OF_BOUNDS(256, 4) ce_pad_table_kernel(CeRowsArgs a) {
 OF_GLOBAL void OF_BOUNDS(256, 2) ce_finish_kernel(CeRowsArgs a) {
     float* red = (float*)of_smem();          // [16 groups][16 rows][2]
     const int tid = of_tid(), r = tid & 15, j = tid >> 4, count = *a.count;
+    if (a.gate && *a.gate == 0) return;
     const long i0 = (long)of_bid_x() * 16;
     if (i0 >= of_ce_live_rows(count)) return;
     const long i = i0 + r;
     float m = oft::CE_LOWEST, s = 0.f;
+    if (a.ref) {
+#pragma unroll 4
+        for (int t = j; t < a.strips; t += 16) s += a.part[(size_t)t * a.part_ld + i];
+        m = a.ref[i];
+    } else
 #pragma unroll 4
     for (int t = j; t < a.strips; t += 16) {
         const f32x2 q = *(const f32x2*)(a.part + ((size_t)t * a.part_ld + i) * 2);
@@ -180,7 +219,10 @@ OF_GLOBAL void OF_BOUNDS(256, 2) ce_finish_kernel(CeRowsArgs a) {
         for (int k = 0; k < 16; ++k) sum += red[(k * 16 + r) * 2 + 1] * of_exp2(red[(k * 16 + r) * 2] - top);
         const float lse = top + of_log2(sum);
         a.lse[i] = i < count ? lse : __builtin_inff();          // behind `count`: exp(z - inf) = 0, rows of D that are zero
-        if (i < count) a.loss_rows[a.row_of[i]] = (lse - a.zlab[i]) * oft::CE_LN2;
+        if (i < count) {
+            a.loss_rows[a.row_of[i]] = (lse - a.zlab[i]) * oft::CE_LN2;
+            if (a.far && lse - a.ref[i] > CE_FAR) *a.far = 1;
+        }
     }
 }
 
@@ -376,7 +418,8 @@ OF_GLOBAL void OF_BOUNDS(256, 4) ce_row_grads_kernel(CeRowsArgs a) {
     if (i < of_ce_live_rows(count)) a.grow[i] = i < count ? a.grad[a.row_of[i]] : 0.f;
 }
 
-// dx[row] = bf16(logit_scale * scale * the sum of acc's parts), zeros for rows without a label; one wave per row
+// dx[row] = bf16(logit_scale * scale * the sum of acc's parts), zeros for rows without a label; one wave per row.  EARLY: acc is E W, and
+// the row's own factor and the label's part join here, in fp32.
 OF_GLOBAL void OF_BOUNDS(256, 4) ce_scatter_kernel(CeRowsArgs a) {
     const int lane = of_tid() & 63;
     const long r = (long)of_bid_x() * 4 + (of_tid() >> 6);
@@ -384,7 +427,17 @@ OF_GLOBAL void OF_BOUNDS(256, 4) ce_scatter_kernel(CeRowsArgs a) {
     const int i = a.slot_of[r], live = of_ce_live_rows(*a.count);
     const int parts = of_ce_splits((live >> 8) * ((a.d + 255) >> 8), a.split_stages);
     const size_t part = (size_t)live * a.d;
-    const float sc = a.logit_scale * of_ce_scale(a.grad, a.by_count, a.count);
+    float sc = a.logit_scale * (a.grow ? a.grow[r] : of_ce_scale(a.grad, a.by_count, a.count));
+    float own = 0.f;
+    const bf16_t* w = a.w;
+    if (a.far && i >= 0 && *a.far == 0) {
+        const float lse = a.lse[i];
+        own = sc * (of_exp2(a.zlab[i] - lse) - 1.0f);
+        sc *= of_exp2(a.ref[i] - lse);
+        w += (size_t)a.lab[i] * a.ldw;
+    } else {
+        w = nullptr;
+    }
     const float* src = i < 0 ? nullptr : a.acc + (size_t)i * a.d;
     bf16_t* dst = a.dx + (size_t)r * a.lddx;
     for (int c = lane * 8; c < a.d; c += 512) {
@@ -400,6 +453,12 @@ OF_GLOBAL void OF_BOUNDS(256, 4) ce_scatter_kernel(CeRowsArgs a) {
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] *= sc;
+            if (w) {
+                float x[8];
+                ofg::unpack8(*(const u32x4*)(w + c), x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] += own * x[e];
+            }
         }
         *(u32x4*)(dst + c) = ofg::pack8(o);
     }
@@ -409,37 +468,15 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 long rows_padded(long rows) { return rows > 0 ? (rows + 255) & ~255l : 256; }
 int depth_padded(int d) { return (d + 63) & ~63; }
 
-// what the forward leaves for the backward
-struct CeState {
-    int *count, *slot_of, *row_of, *lab;
-    float* lse;
-    bf16_t* xc;
-    size_t bytes;
-};
-CeState ce_state(void* base, long rows, int d) {
-    const size_t rp = (size_t)rows_padded(rows);
-    char* at = (char*)base;
-    CeState s{};
-    auto take = [&](size_t n) {
-        char* p = at;
-        at += up256(n);
-        return p;
-    };
-    s.count = (int*)take(4);
-    s.slot_of = (int*)take(rp * 4);
-    s.row_of = (int*)take(rp * 4);
-    s.lab = (int*)take(rp * 4);
-    s.lse = (float*)take(rp * 4);
-    s.xc = (bf16_t*)take(rp * depth_padded(d) * 2);
-    s.bytes = (size_t)(at - (char*)base);
-    return s;
-}
-
 // Vocabulary rows of one backward piece.  D (rows x piece, bf16) is written once and read twice: up to 128 MB it stays in the Infinity
 // Cache; a larger piece saves passes over the fp32 sums of dx.
 int ce_piece(const OfLinearCeArgs& a) {
     long p = a.piece;
     if (p <= 0) p = (128l << 20) / (2 * rows_padded(a.rows));
+    // ... and the products' byte offsets are 32-bit: a piece of the table and a piece of D both stay below 4 GiB
+    const long wide = a.ldw > depth_padded(a.d) ? a.ldw : depth_padded(a.d), tall = rows_padded(a.rows);
+    const long most = ((1l << 31) - 1) / (wide > tall ? wide : tall);
+    if (p > most) p = most;
     p &= ~255l;
     const long all = (a.vocab + 255l) & ~255l;
     if (p < 256) p = 256;
@@ -452,6 +489,38 @@ size_t ce_acc_bytes(const OfLinearCeArgs& a) {
     if (rows > most * rp) rows = most * rp;
     return up256((size_t)(rows > rp ? rows : rp) * a.d * 4);
 }
+// what the forward leaves for the backward
+struct CeState {
+    int *count, *far, *slot_of, *row_of, *lab;
+    float *lse, *ref, *zlab, *acc;          // (the last three: EARLY)
+    bf16_t* xc;
+    size_t bytes;
+};
+CeState ce_state(const OfLinearCeArgs& a) {
+    const size_t rp = (size_t)rows_padded(a.rows);
+    char* at = (char*)a.state;
+    CeState s{};
+    auto take = [&](size_t n) {
+        char* p = at;
+        at += up256(n);
+        return p;
+    };
+    s.count = (int*)take(8);
+    s.far = s.count + 1;
+    s.slot_of = (int*)take(rp * 4);
+    s.row_of = (int*)take(rp * 4);
+    s.lab = (int*)take(rp * 4);
+    s.lse = (float*)take(rp * 4);
+    s.xc = (bf16_t*)take(rp * depth_padded(a.d) * 2);
+    if (a.early_dx) {
+        s.ref = (float*)take(rp * 4);
+        s.zlab = (float*)take(rp * 4);
+        s.acc = (float*)take(ce_acc_bytes(a));
+    }
+    s.bytes = (size_t)(at - (char*)a.state);
+    return s;
+}
+
 size_t ce_table_bytes(const OfLinearCeArgs& a) { return depth_padded(a.d) != a.d ? up256((size_t)a.vocab * depth_padded(a.d) * 2) : 0; }
 
 bool ce_few(long rows, int d) { return rows > 0 && rows <= 16 && d > 0 && (d & 7) == 0 && rows * d <= 1 << 15; }          // (rounded up: 128 KB of x in LDS at most)
@@ -466,10 +535,10 @@ int ce_check(const OfLinearCeArgs* args, bool few = false) {
     if ((a.ldx & 7) || (a.ldw & 7) || ((uintptr_t)a.x & 15) || ((uintptr_t)a.w & 15) || ((uintptr_t)a.state & 15) || ((uintptr_t)a.workspace & 15))
         return OF_E_ALIGN;
     if (few) return 0;
-    if (a.state_bytes < of_linear_ce_state_bytes(a.rows, a.d)) return OF_E_WORKSPACE;
+    if (a.state_bytes < of_linear_ce_state_bytes(args)) return OF_E_WORKSPACE;
     // byte offsets inside a tile's operand windows are 32-bit (gemm_w4m.hip); the weight gradient walks all rows of D and of xc
     const unsigned long long lim = 1ull << 32;
-    if (2ull * 256 * (unsigned long long)a.ldw >= lim || 2ull * (unsigned long long)rows_padded(a.rows) * depth_padded(a.d) >= lim) return OF_E_SHAPE;
+    if (2ull * 256 * (unsigned long long)a.ldw >= lim || 2ull * 256 * (unsigned long long)rows_padded(a.rows) >= lim || 2ull * (unsigned long long)rows_padded(a.rows) * depth_padded(a.d) >= lim) return OF_E_SHAPE;
     return 0;
 }
 
@@ -504,9 +573,28 @@ OfCeGemmArgs ce_logits_args(const OfLinearCeArgs& a, const CeState& st, const bf
     return g;
 }
 
+// dx_acc += D W of table rows [v0, v0 + n)
+OfCeGemmArgs ce_dx_args(const OfLinearCeArgs& a, const CeState& st, const bf16_t* w, long ldw, int v0, int n, const bf16_t* D, float* acc) {
+    OfCeGemmArgs q{};
+    const int piece = ce_piece(a);
+    q.epi = OF_EPI_CE_DX;
+    q.A = D; q.lda = piece;
+    q.B = w + (size_t)v0 * ldw; q.ldb = (int)ldw; q.b_trans = 1;
+    q.b_bytes = ((long)(n - 1) * ldw + depth_padded(a.d)) * 2;
+    q.M = (int)rows_padded(a.rows); q.N = (a.d + 255) & ~255; q.K = (n + 63) & ~63;
+    q.C = acc; q.ldc = a.d; q.beta = v0 ? 1.f : 0.f; q.alpha = 1.f;
+    q.count = st.count; q.n_valid = a.d; q.split_stages = piece / 64;
+    return q;
+}
+
 }  // namespace
 
-extern "C" size_t of_linear_ce_state_bytes(long rows, int d) { return rows > 0 && d > 0 ? ce_state(nullptr, rows, d).bytes : 0; }
+extern "C" size_t of_linear_ce_state_bytes(const OfLinearCeArgs* args) {
+    if (!args || args->rows <= 0 || args->vocab <= 0 || args->d <= 0) return 0;
+    OfLinearCeArgs a = *args;
+    a.state = nullptr;
+    return ce_state(a).bytes;
+}
 
 extern "C" int of_linear_ce_stateless(long rows, int d) { return ce_few(rows, d); }
 
@@ -515,8 +603,9 @@ extern "C" size_t of_linear_ce_workspace_bytes(const OfLinearCeArgs* args, int b
     const OfLinearCeArgs& a = *args;
     const size_t rp = (size_t)rows_padded(a.rows);
     if (!backward && !a.state && ce_few(a.rows, a.d)) return (size_t)a.rows * FEW_WG * 8 + 256;
-    if (!backward) return ce_table_bytes(a) + up256((size_t)(((a.vocab + 255l) / 256) * 2) * rp * 8) + up256(rp * 4);
-    return ce_table_bytes(a) + up256(rp * (size_t)ce_piece(a) * 2) + (a.dx ? ce_acc_bytes(a) : 0) + (a.reduction == OF_CE_NONE ? up256(rp * 4) : 0);
+    const size_t strips = (size_t)((a.vocab + 255l) / 256) * 2, D = up256(rp * (size_t)ce_piece(a) * 2);
+    if (!backward) return ce_table_bytes(a) + up256(strips * rp * 8) + (a.early_dx ? D : up256(rp * 4));
+    return ce_table_bytes(a) + D + (a.dx && !a.early_dx ? ce_acc_bytes(a) : 0) + (a.reduction == OF_CE_NONE && !a.early_dx ? up256(rp * 4) : 0);
 }
 
 template <int MT>
@@ -546,7 +635,7 @@ extern "C" int of_linear_ce_fwd(const OfLinearCeArgs* args, void* stream) {
     if (!a.loss_rows || (a.reduction != OF_CE_NONE && !a.loss)) return OF_E_ARG;
     if (a.workspace_bytes < of_linear_ce_workspace_bytes(args, 0)) return OF_E_WORKSPACE;
     of_stream_t s = (of_stream_t)stream;
-    const CeState st = ce_state(a.state, a.rows, a.d);
+    const CeState st = ce_state(a);
     const long rp = rows_padded(a.rows);
     const bf16_t* w;
     long ldw;
@@ -559,6 +648,10 @@ extern "C" int of_linear_ce_fwd(const OfLinearCeArgs* args, void* stream) {
     r.count = st.count; r.slot_of = st.slot_of; r.row_of = st.row_of; r.lab = st.lab; r.lse = st.lse;
     r.loss_rows = a.loss_rows; r.loss = a.reduction == OF_CE_NONE ? nullptr : a.loss; r.mean = a.reduction == OF_CE_MEAN;
     r.x = a.x; r.ldx = a.ldx; r.xc = st.xc; r.ldxc = depth_padded(a.d); r.d = a.d; r.d_pad = depth_padded(a.d);
+    if (a.early_dx) {
+        r.ref = st.ref; r.far = st.far; r.sc2 = a.logit_scale * oft::CE_LOG2E;
+        r.w = w; r.ldw = ldw;
+    }
     if (a.rows <= CE_FEW_ROWS) {
         rc = of_launch(ce_index_gather_kernel, of_dim3{(unsigned)(rp / 4), 1, 1}, 256, 0, s, r);
     } else {
@@ -568,17 +661,50 @@ extern "C" int of_linear_ce_fwd(const OfLinearCeArgs* args, void* stream) {
     }
     if (rc) return rc;
 
-    OfCeGemmArgs g = ce_logits_args(a, st, w, ldw, 0, a.vocab);
-    g.epi = OF_EPI_CE_LSE;
-    g.part = (float*)ws; g.part_ld = rp;
-    r.strips = g.N / 128;
-    g.zlab = (float*)(ws + up256((size_t)r.strips * rp * 8));
-    rc = of_gemm_w4m_ce(g, s);
+    r.strips = (int)((a.vocab + 255l) / 256) * 2;
+    r.part_ld = rp;
+    r.part = (float*)ws;
+    if (a.early_dx) {
+        bf16_t* D = (bf16_t*)(ws + up256((size_t)r.strips * rp * 8));
+        r.zlab = st.zlab;
+        const int piece = ce_piece(a);
+        for (int v0 = 0; v0 < a.vocab; v0 += piece) {
+            const int n = a.vocab - v0 < piece ? a.vocab - v0 : piece;
+            OfCeGemmArgs g = ce_logits_args(a, st, w, ldw, v0, n);
+            g.epi = OF_EPI_CE_EARLY;
+            g.lse = st.ref; g.C = D; g.ldc = piece;
+            g.part = (float*)ws; g.part_ld = rp; g.zlab = st.zlab;
+            rc = of_gemm_w4m_ce(g, s);
+            if (rc) return rc;
+            rc = of_gemm_w4m_ce(ce_dx_args(a, st, w, ldw, v0, n, D, st.acc), s);
+            if (rc) return rc;
+        }
+    } else {
+        OfCeGemmArgs g = ce_logits_args(a, st, w, ldw, 0, a.vocab);
+        g.epi = OF_EPI_CE_LSE;
+        g.part = (float*)ws; g.part_ld = rp;
+        g.zlab = (float*)(ws + up256((size_t)r.strips * rp * 8));
+        r.zlab = g.zlab;
+        rc = of_gemm_w4m_ce(g, s);
+        if (rc) return rc;
+    }
+    if (!a.early_dx && rp * r.strips <= CE_FEW_PARTS) return of_launch(ce_finish_reduce_kernel, of_dim3{1, 1, 1}, CE_THREADS, CE_THREADS * sizeof(float), s, r);
+    const of_dim3 grid{(unsigned)(rp / 16), 1, 1};
+    const size_t lds = 16 * 16 * 2 * sizeof(float);
+    rc = of_launch(ce_finish_kernel, grid, 256, lds, s, r);
     if (rc) return rc;
-    r.part = g.part; r.part_ld = rp; r.zlab = g.zlab;
-    if (rp * r.strips <= CE_FEW_PARTS) return of_launch(ce_finish_reduce_kernel, of_dim3{1, 1, 1}, CE_THREADS, CE_THREADS * sizeof(float), s, r);
-    rc = of_launch(ce_finish_kernel, of_dim3{(unsigned)(rp / 16), 1, 1}, 256, 16 * 16 * 2 * sizeof(float), s, r);
-    if (rc || a.reduction == OF_CE_NONE) return rc;
+    if (a.early_dx) {          // some loss above CE_FAR: the statistics with a maximum, for every row
+        OfCeGemmArgs g = ce_logits_args(a, st, w, ldw, 0, a.vocab);
+        g.epi = OF_EPI_CE_LSE;
+        g.part = (float*)ws; g.part_ld = rp; g.zlab = st.zlab;
+        g.gate = r.gate = st.far;
+        rc = of_gemm_w4m_ce(g, s);
+        if (rc) return rc;
+        r.ref = nullptr; r.far = nullptr;
+        rc = of_launch(ce_finish_kernel, grid, 256, lds, s, r);
+        if (rc) return rc;
+    }
+    if (a.reduction == OF_CE_NONE) return 0;
     return of_launch(ce_reduce_kernel, of_dim3{1, 1, 1}, CE_THREADS, CE_THREADS * sizeof(float), s, r);
 }
 
@@ -586,16 +712,14 @@ extern "C" int of_linear_ce_bwd(const OfLinearCeArgs* args, void* stream) {
     const int bad = ce_check(args);
     if (bad) return bad;
     const OfLinearCeArgs& a = *args;
-    if (!a.grad || (!a.dx && !a.dw)) return OF_E_ARG;
+    if (!a.grad || (!a.dx && !a.dw) || (a.early_dx && (!a.dx || a.dw))) return OF_E_ARG;
     if ((a.dx && a.lddx < a.d) || (a.dw && a.lddw < a.d)) return OF_E_ARG;
     if ((a.lddx & 7) || (a.lddw & 7) || ((uintptr_t)a.dx & 15) || ((uintptr_t)a.dw & 15)) return OF_E_ALIGN;
     if (a.workspace_bytes < of_linear_ce_workspace_bytes(args, 1)) return OF_E_WORKSPACE;
     of_stream_t s = (of_stream_t)stream;
-    const CeState st = ce_state(a.state, a.rows, a.d);
+    const CeState st = ce_state(a);
     const long rp = rows_padded(a.rows);
     const int piece = ce_piece(a), dp = depth_padded(a.d), d256 = (a.d + 255) & ~255;
-    // every operand window of the pieces' products is checked before the first launch
-    if (2ull * (unsigned long long)rp * piece >= (1ull << 32) || 2ull * (unsigned long long)piece * (unsigned long long)a.ldw >= (1ull << 32)) return OF_E_SHAPE;
     const bf16_t* w;
     long ldw;
     char* ws;
@@ -603,8 +727,8 @@ extern "C" int of_linear_ce_bwd(const OfLinearCeArgs* args, void* stream) {
     if (rc) return rc;
     bf16_t* D = (bf16_t*)ws;
     ws += up256((size_t)rp * piece * 2);
-    float* acc = nullptr;
-    if (a.dx) {
+    float* acc = st.acc;
+    if (a.dx && !acc) {
         acc = (float*)ws;
         ws += ce_acc_bytes(a);
     }
@@ -612,11 +736,16 @@ extern "C" int of_linear_ce_bwd(const OfLinearCeArgs* args, void* stream) {
     CeRowsArgs r{};
     r.rows = a.rows; r.count = st.count; r.slot_of = st.slot_of; r.row_of = st.row_of;
     r.d = a.d; r.acc = acc; r.split_stages = piece / 64; r.dx = a.dx; r.lddx = a.lddx;
-    if (a.reduction == OF_CE_NONE) {
+    float* grow = nullptr;
+    if (a.early_dx) {          // the rows' own gradients join at the end
+        r.far = st.far; r.ref = st.ref; r.zlab = st.zlab; r.lse = st.lse; r.lab = st.lab; r.w = w; r.ldw = ldw;
+        if (a.reduction == OF_CE_NONE) r.grow = const_cast<float*>(a.grad);
+    } else if (a.reduction == OF_CE_NONE) {
         r.grad = a.grad;
-        r.grow = (float*)ws;
+        r.grow = grow = (float*)ws;
         rc = of_launch(ce_row_grads_kernel, of_dim3{(unsigned)((rp + 255) / 256), 1, 1}, 256, 0, s, r);
         if (rc) return rc;
+        r.grow = nullptr;
     }
     const float* gscale = a.reduction == OF_CE_NONE ? nullptr : a.grad;
     const int by_count = a.reduction == OF_CE_MEAN;
@@ -625,18 +754,13 @@ extern "C" int of_linear_ce_bwd(const OfLinearCeArgs* args, void* stream) {
         const int n = a.vocab - v0 < piece ? a.vocab - v0 : piece;
         OfCeGemmArgs g = ce_logits_args(a, st, w, ldw, v0, n);
         g.epi = OF_EPI_CE_DLOGIT;
-        g.C = D; g.ldc = piece; g.grow = r.grow;
+        g.C = D; g.ldc = piece; g.grow = grow;
+        if (a.early_dx) g.gate = st.far;
         rc = of_gemm_w4m_ce(g, s);
         if (rc) return rc;
         if (a.dx) {
-            OfCeGemmArgs q{};
-            q.epi = OF_EPI_CE_DX;
-            q.A = D; q.lda = piece;
-            q.B = w + (size_t)v0 * ldw; q.ldb = (int)ldw; q.b_trans = 1;
-            q.b_bytes = ((long)(n - 1) * ldw + dp) * 2;
-            q.M = (int)rp; q.N = d256; q.K = (n + 63) & ~63;
-            q.C = acc; q.ldc = a.d; q.beta = v0 ? 1.f : 0.f; q.alpha = 1.f;
-            q.count = st.count; q.n_valid = a.d; q.split_stages = piece / 64;
+            OfCeGemmArgs q = ce_dx_args(a, st, w, ldw, v0, n, D, acc);
+            if (a.early_dx) q.gate = st.far;
             rc = of_gemm_w4m_ce(q, s);
             if (rc) return rc;
         }

@@ -97,6 +97,7 @@ class OfLinearCeArgs(C.Structure):
         ("dx", vp), ("lddx", C.c_long),
         ("dw", vp), ("lddw", C.c_long),
         ("piece", C.c_int),
+        ("early_dx", C.c_int),
         ("workspace", vp), ("workspace_bytes", C.c_size_t),
     ]
 
@@ -156,7 +157,7 @@ PROTOTYPES = {
     "of_add_embs": (C.c_int, [vp, C.c_int, vp, C.c_long, C.c_int, vp, C.c_long, C.c_int, vp, C.c_long, C.c_int, vp]),
     "of_ce_fwd": (C.c_int, [vp, C.c_int, C.c_long, vp, C.c_longlong, C.c_long, C.c_int, vp, vp, vp]),
     "of_ce_bwd": (C.c_int, [vp, C.c_int, C.c_long, vp, C.c_longlong, C.c_long, C.c_int, vp, vp, vp, C.c_long, vp]),
-    "of_linear_ce_state_bytes": (C.c_size_t, [C.c_long, C.c_int]),
+    "of_linear_ce_state_bytes": (C.c_size_t, [C.POINTER(OfLinearCeArgs)]),
     "of_linear_ce_stateless": (C.c_int, [C.c_long, C.c_int]),
     "of_linear_ce_workspace_bytes": (C.c_size_t, [C.POINTER(OfLinearCeArgs), C.c_int]),
     "of_linear_ce_fwd": (C.c_int, [C.POINTER(OfLinearCeArgs), vp]),

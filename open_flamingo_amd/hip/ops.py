@@ -452,57 +452,53 @@ class Ops:
                                      self._stream()), "of_ce_bwd")
 
     # ------------------------------------------------------------------ the same loss without the logits
-    def _linear_ce_args(self, x, w, labels, state, *, ignore_index, logit_scale, reduction, piece=0):
-        rows, d = x.shape
-        if x.dtype != BF16 or w.dtype != BF16:
+    def _linear_ce_args(self, x, w, labels, *, ignore_index, logit_scale, reduction, piece, early):
+        (rows, d), (ldx, cx), (ldw, cw) = x.shape, x.stride(), w.stride()
+        if x.dtype is not BF16 or w.dtype is not BF16:
             raise TypeError(f"linear_ce takes bfloat16 hidden states and table, got {x.dtype} and {w.dtype}")
         if w.dim() != 2 or w.shape[1] != d:
             raise ValueError(f"hidden states {tuple(x.shape)} and table {tuple(w.shape)} do not fit")
-        if labels.dtype != torch.int64 or not labels.is_contiguous() or labels.numel() != rows:
+        if labels.dtype is not torch.int64 or not labels.is_contiguous() or labels.numel() != rows:
             raise ValueError("labels: one int64 per row, contiguous")
-        assert x.stride(1) == 1 and w.stride(1) == 1 and (state is None or (state.dtype == torch.uint8 and state.is_contiguous()))
-        a = abi.OfLinearCeArgs()
-        a.x, a.ldx = x.data_ptr(), x.stride(0) if rows > 1 else max(x.stride(0), d)
-        a.w, a.ldw = w.data_ptr(), w.stride(0) if w.shape[0] > 1 else max(w.stride(0), d)
-        a.labels, a.ignore_index = labels.data_ptr(), ignore_index
-        a.rows, a.vocab, a.d = rows, w.shape[0], d
-        a.logit_scale, a.reduction, a.piece = logit_scale, reduction, piece
-        if state is not None:
-            a.state, a.state_bytes = state.data_ptr(), state.numel()
+        assert cx == 1 and cw == 1
+        a = abi.OfLinearCeArgs(x=x.data_ptr(), ldx=max(ldx, d), w=w.data_ptr(), ldw=max(ldw, d), labels=labels.data_ptr(), ignore_index=ignore_index, rows=rows,
+                               vocab=w.shape[0], d=d, logit_scale=logit_scale, reduction=reduction, piece=piece, early_dx=early)
         return a
 
     def _linear_ce_workspace(self, a, backward, device):
-        ws = torch.empty(self.lib.of_linear_ce_workspace_bytes(C.byref(a), backward), dtype=torch.uint8, device=device)
+        ws = torch.empty(self.lib.of_linear_ce_workspace_bytes(a, backward), dtype=torch.uint8, device=device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
         return ws
 
-    def linear_ce_state(self, rows, d, device, grad=True):
-        """what linear_ce_fwd leaves for linear_ce_bwd (of_linear_ce_state_bytes); grad = False, no backward to follow: None where none is needed"""
-        if not grad and self.lib.of_linear_ce_stateless(rows, d):
-            return None
-        return torch.empty(self.lib.of_linear_ce_state_bytes(rows, d), dtype=torch.uint8, device=device)
-
-    def linear_ce_fwd(self, x, w, labels, state, loss_rows, loss=None, *, ignore_index=-100, logit_scale=1.0, reduction=abi.CE_MEAN):
-        """loss_rows (rows, fp32) and, for CE_MEAN / CE_SUM, loss (1, fp32) of softmax cross entropy over logit_scale * x @ w.T."""
-        a = self._linear_ce_args(x, w, labels, state, ignore_index=ignore_index, logit_scale=logit_scale, reduction=reduction)
-        assert loss_rows.dtype == F32 and loss_rows.is_contiguous() and loss_rows.numel() == a.rows
-        assert loss is None or (loss.dtype == F32 and loss.numel() == 1)
+    def linear_ce_fwd(self, x, w, labels, loss_rows, loss=None, *, ignore_index=-100, logit_scale=1.0, reduction=abi.CE_MEAN, piece=0, need=(False, False)):
+        """loss_rows (rows, fp32) and, for CE_MEAN / CE_SUM, loss (1, fp32) of softmax cross entropy over logit_scale * x @ w.T.  Returns the
+        state that linear_ce_bwd takes (with the same arguments); need: which of (dx, dw) will be asked of it."""
+        a = self._linear_ce_args(x, w, labels, ignore_index=ignore_index, logit_scale=logit_scale, reduction=reduction, piece=piece, early=int(need[0] and not need[1]))
+        assert loss_rows.dtype is F32 and loss_rows.is_contiguous() and loss_rows.numel() == a.rows
+        assert loss is None or (loss.dtype is F32 and loss.numel() == 1)
         a.loss_rows, a.loss = loss_rows.data_ptr(), _p(loss)
+        state = None
+        if need[0] or need[1] or not self.lib.of_linear_ce_stateless(a.rows, a.d):
+            state = torch.empty(self.lib.of_linear_ce_state_bytes(a), dtype=torch.uint8, device=x.device)
+            a.state, a.state_bytes = state.data_ptr(), state.numel()
         ws = self._linear_ce_workspace(a, 0, x.device)          # noqa: F841 (alive until the launches are enqueued)
-        self._chk(self.lib.of_linear_ce_fwd(C.byref(a), self._stream()), "of_linear_ce_fwd")
+        self._chk(self.lib.of_linear_ce_fwd(a, self._stream()), "of_linear_ce_fwd")
+        return state
 
     def linear_ce_bwd(self, x, w, labels, state, grad, dx=None, dw=None, *, ignore_index=-100, logit_scale=1.0, reduction=abi.CE_MEAN, piece=0):
-        """dx and / or dw (bf16) from the forward's state; grad: fp32 on the device, one value or (CE_NONE) one per row."""
-        a = self._linear_ce_args(x, w, labels, state, ignore_index=ignore_index, logit_scale=logit_scale, reduction=reduction, piece=piece)
-        assert grad.dtype == F32 and grad.is_contiguous() and grad.numel() == (a.rows if reduction == abi.CE_NONE else 1)
-        a.grad = grad.data_ptr()
-        for t, like, name in ((dx, x, "dx"), (dw, w, "dw")):
-            if t is not None:
-                assert t.dtype == BF16 and t.shape == like.shape and t.stride(1) == 1, name
-                setattr(a, name, t.data_ptr())
-                setattr(a, "ld" + name, max(t.stride(0), a.d))
+        """dx and / or dw (bf16), as announced to the forward; grad: fp32 on the device, one value or (CE_NONE) one per row."""
+        a = self._linear_ce_args(x, w, labels, ignore_index=ignore_index, logit_scale=logit_scale, reduction=reduction, piece=piece,
+                                 early=int(dx is not None and dw is None))
+        assert grad.dtype is F32 and grad.is_contiguous() and grad.numel() == (a.rows if reduction == abi.CE_NONE else 1)
+        a.state, a.state_bytes, a.grad = state.data_ptr(), state.numel(), grad.data_ptr()
+        if dx is not None:
+            assert dx.dtype is BF16 and dx.shape == x.shape and dx.stride(1) == 1
+            a.dx, a.lddx = dx.data_ptr(), max(dx.stride(0), a.d)
+        if dw is not None:
+            assert dw.dtype is BF16 and dw.shape == w.shape and dw.stride(1) == 1
+            a.dw, a.lddw = dw.data_ptr(), max(dw.stride(0), a.d)
         ws = self._linear_ce_workspace(a, 1, x.device)          # noqa: F841
-        self._chk(self.lib.of_linear_ce_bwd(C.byref(a), self._stream()), "of_linear_ce_bwd")
+        self._chk(self.lib.of_linear_ce_bwd(a, self._stream()), "of_linear_ce_bwd")
 
     # ------------------------------------------------------------------ lookup in a vocabulary table
     def embedding_fwd(self, ids, table, out, scale=1.0):

@@ -33,35 +33,33 @@ def _on(t):
     return nullcontext() if at < 0 or at == torch.cuda.current_device() else torch.cuda.device(at)
 
 
-def _linear_ce(hidden, table, labels, kw, ops, grad):
+def _linear_ce(hidden, table, labels, kw, ops, need):
     """(loss, what a backward needs)"""
     x, w = _rows16(hidden), _rows16(table)
-    rows, d = x.shape
-    loss_rows = torch.empty(rows, dtype=F32, device=x.device)
+    loss_rows = torch.empty(x.shape[0], dtype=F32, device=x.device)
     loss = torch.empty((), dtype=F32, device=x.device) if kw["reduction"] != abi.CE_NONE else None
-    state = ops.linear_ce_state(rows, d, x.device, grad)
-    ops.linear_ce_fwd(x, w, labels, state, loss_rows, loss, **kw)
+    state = ops.linear_ce_fwd(x, w, labels, loss_rows, loss, need=need, **kw)
     return loss_rows if loss is None else loss, (x, w, labels, state)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, table, labels, kw, piece, ops):
-        loss, saved = _linear_ce(hidden, table, labels, kw, ops, True)
+    def forward(ctx, hidden, table, labels, kw, ops):
+        ctx.need = ctx.needs_input_grad[:2]
+        loss, saved = _linear_ce(hidden, table, labels, kw, ops, ctx.need)
         ctx.save_for_backward(*saved)
-        ctx.kw, ctx.piece, ctx.ops = kw, piece, ops
+        ctx.kw, ctx.ops = kw, ops
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         x, w, labels, state = ctx.saved_tensors
-        need_x, need_w = ctx.needs_input_grad[:2]
-        dx = torch.empty(x.shape, dtype=BF16, device=x.device) if need_x else None
-        dw = torch.empty(w.shape, dtype=BF16, device=w.device) if need_w else None
+        dx = torch.empty(x.shape, dtype=BF16, device=x.device) if ctx.need[0] else None
+        dw = torch.empty(w.shape, dtype=BF16, device=w.device) if ctx.need[1] else None
         with _on(x):
-            ctx.ops.linear_ce_bwd(x, w, labels, state, g.to(F32).contiguous(), dx, dw, piece=ctx.piece, **ctx.kw)
-        return dx, dw, None, None, None, None
+            ctx.ops.linear_ce_bwd(x, w, labels, state, g.to(F32).contiguous(), dx, dw, **ctx.kw)
+        return dx, dw, None, None, None
 
 
 def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction="mean", logit_scale=1.0, piece=0, ops=None):
@@ -71,7 +69,7 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
     hidden (..., d) and table (vocabulary, d): bfloat16, or any floating type under bf16 autocast (cast as ``F.linear`` casts); d a
     multiple of 8.  labels (...): int64, already shifted.  reduction "mean" (over the labels that count: NaN without any), "sum" or
     "none" (one fp32 loss per label, 0 where ignored).  A label outside the vocabulary that is not ``ignore_index`` makes the loss NaN and
-    has no gradient.  Gradients come in bfloat16 for both operands, through fp32 sums; ``piece``: vocabulary rows the backward
+    has no gradient.  Where the table has no gradient the forward prepares the hidden states' one from the same product.  Gradients come in bfloat16 for both operands, through fp32 sums; ``piece``: vocabulary rows the backward
     holds a logits gradient of at a time (0: chosen, 128 MB of it)."""
     if reduction not in _REDUCTION:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {reduction!r}")
@@ -79,6 +77,8 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
         raise ValueError(f"labels {tuple(labels.shape)} do not fit hidden states {tuple(hidden.shape)}")
     if table.dim() != 2 or table.shape[1] != hidden.shape[-1] or table.shape[0] == 0:
         raise ValueError(f"table {tuple(table.shape)} does not fit hidden states {tuple(hidden.shape)}")
+    if (labels.numel() + 255) // 256 * 256 * ((hidden.shape[-1] + 63) // 64 * 64) >= 1 << 31:
+        raise ValueError(f"{labels.numel()} rows of {hidden.shape[-1]}: the hidden states of a call must stay below 2^31 elements; split the batch")
     if hidden.shape[-1] % 8:
         raise ValueError(f"the hidden size must be a multiple of 8, got {hidden.shape[-1]}")
     if labels.dtype != torch.int64:
@@ -97,12 +97,12 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
     if x.shape[0] == 0:          # no rows: torch's values, zero gradients
         zero = (hidden.sum() + table[:0].sum()).to(F32)
         return zero.new_zeros(labels.shape) if reduction == "none" else zero / 0.0 if reduction == "mean" else zero
-    kw = dict(ignore_index=int(ignore_index), logit_scale=float(logit_scale), reduction=_REDUCTION[reduction])
+    kw = dict(ignore_index=int(ignore_index), logit_scale=float(logit_scale), reduction=_REDUCTION[reduction], piece=int(piece))
     with _on(x):
         if torch.is_grad_enabled() and (x.requires_grad or table.requires_grad):
-            out = _LinearCrossEntropy.apply(x, table, y, kw, int(piece), ops)
+            out = _LinearCrossEntropy.apply(x, table, y, kw, ops)
         else:
-            out = _linear_ce(x, table, y, kw, ops, False)[0]
+            out = _linear_ce(x, table, y, kw, ops, (False, False))[0]
     return out.view(labels.shape) if reduction == "none" else out
 
 
@@ -179,6 +179,10 @@ def _runs_here(t):
     return True
 
 
+def _keeps_all(logits_to_keep):
+    return isinstance(logits_to_keep, int) and logits_to_keep == 0
+
+
 def _embedding_forward(self, ids):
     if ids.dtype == torch.int64 and _runs_here(self.weight):
         return embedding_lookup(ids, self.weight, padding_idx=self.padding_idx)
@@ -191,10 +195,13 @@ class _VocabLossMixin:
     cover (a head with a bias, ``logits_to_keep``, other loss arguments, operands that are not bf16 or under bf16 autocast, the two-row mode of
     train/sparse_rows.py, whose tap sits behind the logits) takes the LM's own path."""
 
-    def _of_takes(self, labels, kwargs):
+    def _of_takes(self, args, kwargs):
+        labels = kwargs.get("labels")
+        if len(args) > 1:          # (what the second positional argument is differs from LM to LM)
+            return False
         head = self.get_output_embeddings()
         w = getattr(head, "weight", None)
-        if labels is None or w is None or getattr(head, "bias", None) is not None or kwargs.get("logits_to_keep") or not _runs_here(w):
+        if labels is None or w is None or w.shape[1] % 8 or getattr(head, "bias", None) is not None or not _keeps_all(kwargs.get("logits_to_keep", 0)) or not _runs_here(w):
             return False
         if any(kwargs.get(k) is not None for k in ("num_items_in_batch", "shift_labels", "ignore_index")) or getattr(w, "_of_trained_rows", None) is not None:
             return False
@@ -202,21 +209,23 @@ class _VocabLossMixin:
         amp = torch.is_autocast_enabled(dev) and torch.get_autocast_dtype(dev) == BF16
         return amp or w.dtype == BF16
 
-    def forward(self, input_ids=None, attention_mask=None, labels=None, **kwargs):
-        if not self._of_takes(labels, kwargs):
-            return super().forward(input_ids=input_ids, attention_mask=attention_mask, labels=labels, **kwargs)
+    def forward(self, *args, **kwargs):
+        if not self._of_takes(args, kwargs):
+            return super().forward(*args, **kwargs)
+        labels = kwargs.pop("labels")
+        kwargs.pop("logits_to_keep", None)
         seen = []
         hook = self.base_model.register_forward_hook(lambda mod, args, out: seen.append(out[0]))
         try:          # the LM's own forward with no position for the head: hidden states, cache and all the rest as it makes them
             none = torch.empty(0, dtype=torch.int64, device=labels.device)
-            out = super().forward(input_ids=input_ids, attention_mask=attention_mask, logits_to_keep=none, **kwargs)
+            out = super().forward(*args, logits_to_keep=none, **kwargs)
         finally:
             hook.remove()
         w = self.get_output_embeddings().weight
         ahead = torch.nn.functional.pad(labels.to(seen[-1].device), (0, 1), value=-100)[..., 1:]          # position i predicts token i + 1
         loss = linear_cross_entropy(seen[-1], w, ahead.to(torch.int64))
-        if isinstance(out, tuple):
-            return (loss,) + out[1:]
+        if isinstance(out, tuple):          # (logits, ...) without labels: (loss, logits, ...) with
+            return (loss, None) + out[1:]
         return type(out)(loss=loss, **{k: v for k, v in out.items() if k != "logits"})
 
 

@@ -13,7 +13,7 @@ def ce_inputs(rows, d, vocab, seed=0, drop=0.3, ignore=-100, device="cpu"):
     return x.to(device), w.to(device), y.to(device)
 
 
-def ce_reference(x, w, y, upstream, reduction, ignore=-100, scale=1.0):
+def ce_reference(x, w, y, upstream, reduction, ignore=-100, scale=1.0, early=False):
     """(loss, dx, dw, how far dx may be off, how far dw) in 64 bits.
 
     The operands are bf16 values, products exact in fp32, sums in fp32: that part is below 1e-5 of the sums of magnitudes.  An entry of
@@ -28,17 +28,22 @@ def ce_reference(x, w, y, upstream, reduction, ignore=-100, scale=1.0):
     D = lp.exp()
     D[torch.arange(len(y), device=y.device), y.clamp(min=0)] -= 1
     g = upstream.double()[:, None] if reduction == "none" else upstream.double() / (max(n, 1) if reduction == "mean" else 1)
-    D = torch.where(keep[:, None], D * g * scale, 0.0)
+    one = torch.zeros_like(D)
+    one[torch.arange(len(y), device=y.device), y.clamp(min=0)] = 1
+    D, one = (torch.where(keep[:, None], t * g * scale, 0.0) for t in (D, one))
     dx, dw = D @ wd, D.t() @ xd
     tol = BF16_HALF + 1e-5
-    return loss, dx, dw, tol * (dx.abs() + D.abs() @ wd.abs()) + 1e-30, tol * (dw.abs() + D.abs().t() @ xd.abs()) + 1e-30
+    bx = tol * (dx.abs() + D.abs() @ wd.abs()) + 1e-30
+    if early:          # the label's p - 1 is formed in fp32 from a logit and a log-sum-exp of z log2 e: 8 half steps of 2^-24 of those
+        bx = bx + 2.0 ** -21 * (z.abs().amax(1, keepdim=True) * 1.4427).clamp(min=1) * (one.abs() @ wd.abs())
+    return loss, dx, dw, bx, tol * (dw.abs() + D.abs().t() @ xd.abs()) + 1e-30
 
 
-def ce_check(run, rows, d, vocab, reduction, drop, scale=1.0, seed=0, device="cpu"):
-    """run(x, w, y, upstream) -> (loss, dx, dw)"""
+def ce_check(run, rows, d, vocab, reduction, drop, scale=1.0, seed=0, device="cpu", early=False):
+    """run(x, w, y, upstream) -> (loss, dx, dw); early: dx alone was asked for"""
     x, w, y = ce_inputs(rows, d, vocab, drop=drop, seed=seed, device=device)
     up = torch.rand(rows, generator=torch.Generator().manual_seed(1)).to(device) + 0.5 if reduction == "none" else torch.tensor(0.75, device=device)
-    loss, dx, dw, bx, bw = ce_reference(x, w, y, up, reduction, scale=scale)
+    loss, dx, dw, bx, bw = ce_reference(x, w, y, up, reduction, scale=scale, early=early)
     got, gx, gw = run(x, w, y, up)
     if bool((y != -100).any()) or reduction != "mean":
         assert ((got.double() - loss).abs() <= 1e-5 * loss.abs().clamp(min=1)).all(), (got, loss)
