@@ -29,7 +29,7 @@ struct EmbArgs {
     unsigned *key_in, *pos_in, *key_out, *pos_out; int shift; int from_ids; int nb;
     int* hist;
     const unsigned *key, *pos; int chunk; long chunks; float* part;
-    int passes;
+    int passes; int cap;
 };
 
 OF_DEV unsigned emb_key(const EmbArgs& a, long i) {
@@ -149,7 +149,6 @@ OF_DEV void emb_fill(const EmbArgs& a, long block, long blocks, int tid, int nth
 // Workgroup 0 sorts all positions (at most SMALL_MAX) in LDS: two lists of key << 14 | position (a key has 18 bits at most: larger
 // vocabularies take the launches below), 16-bit counters of every wave (a place is below 16384), the scan.  The others clear the table.
 constexpr int SMALL_WAVES = SMALL_THREADS / 64, SMALL_ITERS = SMALL_MAX / SMALL_THREADS;
-constexpr size_t SMALL_LDS = 2 * SMALL_MAX * 4 + SMALL_WAVES * BINS * 2 + BINS * 4;
 OF_GLOBAL void OF_BOUNDS(SMALL_THREADS, 1) emb_sort_small_kernel(EmbArgs a) {
     const int tid = of_tid(), lane = tid & 63, wave = tid >> 6;
     if (of_bid_x() > 0) {
@@ -157,8 +156,8 @@ OF_GLOBAL void OF_BOUNDS(SMALL_THREADS, 1) emb_sort_small_kernel(EmbArgs a) {
         return;
     }
     unsigned* from = (unsigned*)of_smem();
-    unsigned* to = from + SMALL_MAX;
-    unsigned short* cnt = (unsigned short*)(to + SMALL_MAX);
+    unsigned* to = from + a.cap;
+    unsigned short* cnt = (unsigned short*)(to + a.cap);
     int* cum = (int*)(cnt + SMALL_WAVES * BINS);
     const int n = (int)a.n;
     const int iters = (n + SMALL_THREADS - 1) / SMALL_THREADS;          // 64 elements of every wave at a time; a wave's part is consecutive
@@ -498,7 +497,11 @@ extern "C" int of_embedding_bwd(const long long* ids, long n, const void* dy, in
     int rc, in = 0;
     if (emb_small(n, vocab)) {
         a.key_out = key[0]; a.pos_out = pos[0];
-        rc = of_launch(emb_sort_small_kernel, of_dim3{(unsigned)(1 + (fill < 512 ? fill : 512)), 1, 1}, SMALL_THREADS, SMALL_LDS, s, a);
+        a.cap = (int)(n + 63) / 64 * 64;
+        const size_t lds = 2 * (size_t)a.cap * 4 + SMALL_WAVES * BINS * 2 + BINS * 4;
+        // 256 workgroups sweep the table in windows of 4 MB: 766 MB cleared beside a sort of 39 positions takes 138 us in all; 255, 511
+        // and 1022 of them, whose windows do not end at a power of two, take 166, 155 and 170, 512 (two to a compute unit) 159
+        rc = of_launch(emb_sort_small_kernel, of_dim3{(unsigned)(1 + (fill < 256 ? fill : 256)), 1, 1}, SMALL_THREADS, lds, s, a);
         if (rc) return rc;
     } else {
         for (int p = 0; p < a.passes; ++p) {

@@ -47,13 +47,13 @@ constexpr int MT_NORM_MAX = 196;            // the norm needs less of a tensor: 
 struct MtNormArgs {
     int n;
     int chunk_end[MT_NORM_MAX];
-    float* parts;
+    double* parts;
     unsigned long long g[MT_NORM_MAX];      // address, plus 1 for bf16
     long count[MT_NORM_MAX];
 };
 static_assert(sizeof(MtArgs) <= 4096 && sizeof(MtNormArgs) <= 4096, "kernel arguments");
 struct MtBeginArgs {
-    const float* parts; long count;
+    const double* parts; long count;
     float max_norm; double beta1, beta2;
     int step; int* applied;
     MtStep* out; float* sumsq;
@@ -114,13 +114,25 @@ OF_DEV void mt_store_codes(void* base, bool vec, long i, long n, unsigned u) {
 }
 
 // ------------------------------------------------------------------------------------------------ the norm
+// 256 lanes' values in a fixed order, the result in thread 0
+OF_DEV double mt_sum64(double s, double* red, int tid) {
+    red[tid] = s;
+    of_sync();
+    for (int o = 128; o >= 1; o >>= 1) {
+        if (tid < o) red[tid] += red[tid + o];
+        of_sync();
+    }
+    return red[0];
+}
+// The sum of squares in 64 bits: the pass waits for memory, and the clip factor then does not depend on how the elements are cut into
+// workgroups (8-bit moments make a rounding of the factor visible: one code in a few million).
 // Workgroup b of MT_PARTS takes chunks b, b + MT_PARTS, ... (32 KB each: the grid as a whole walks memory front to back -- with a long run of
 // its own for every workgroup the same pass read 3.6 TB/s); which slot sums which elements depends on the sizes alone
 OF_GLOBAL void OF_BOUNDS(256, 4) mt_sumsq_kernel(MtNormArgs a) {
-    float* red = (float*)of_smem();
+    double* red = (double*)of_smem();
     const int tid = of_tid(), all = a.chunk_end[a.n - 1];
     int k = 0;
-    float s = 0.f, s2 = 0.f;
+    double s = 0.0, s2 = 0.0;
     for (int c = of_bid_x(); c < all; c += MT_PARTS) {
         while (a.chunk_end[k] <= c) ++k;
         const unsigned long long at = a.g[k];
@@ -132,30 +144,28 @@ OF_GLOBAL void OF_BOUNDS(256, 4) mt_sumsq_kernel(MtNormArgs a) {
 #pragma unroll
         for (int u = 0; u < 8; ++u) g[u] = mt_load(g0, bf16, vec, i + u * 1024, n);
 #pragma unroll
-        for (int u = 0; u < 8; u += 2) {
-            s += (g[u][0] * g[u][0] + g[u][1] * g[u][1]) + (g[u][2] * g[u][2] + g[u][3] * g[u][3]);
-            s2 += (g[u + 1][0] * g[u + 1][0] + g[u + 1][1] * g[u + 1][1]) + (g[u + 1][2] * g[u + 1][2] + g[u + 1][3] * g[u + 1][3]);
-        }
+        for (int u = 0; u < 8; u += 2)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double x = (double)g[u][e], y = (double)g[u + 1][e];
+                s = __builtin_fma(x, x, s);
+                s2 = __builtin_fma(y, y, s2);
+            }
     }
-    s += s2;
-    s = of_wave_sum(s);
-    if ((tid & 63) == 0) red[tid >> 6] = s;
-    of_sync();
-    if (tid == 0) a.parts[of_bid_x()] = (red[0] + red[1]) + (red[2] + red[3]);
+    s = mt_sum64(s + s2, red, tid);
+    if (tid == 0) a.parts[of_bid_x()] = s;
 }
 
 // one workgroup: the partial sums in a fixed order, then everything a step needs once -- bias corrections in 64 bits (1 - 0.999^t loses
 // four digits in 32 at small t).  `applied` counts the steps that were not left out.
 OF_GLOBAL void OF_BOUNDS(256, 1) mt_begin_kernel(MtBeginArgs a) {
-    float* red = (float*)of_smem();
+    double* red = (double*)of_smem();
     const int tid = of_tid();
-    float s = 0.f;
+    double s = 0.0;
     for (long i = tid; i < a.count; i += 256) s += a.parts[i];
-    s = of_wave_sum(s);
-    if ((tid & 63) == 0) red[tid >> 6] = s;
-    of_sync();
+    s = mt_sum64(s, red, tid);
     if (tid == 0) {
-        const float sum = (red[0] + red[1]) + (red[2] + red[3]), norm = sqrtf(sum);
+        const float sum = (float)s, norm = (float)sqrt(s);
         const bool finite = norm < 3.0e38f;
         *a.sumsq = sum;
         int t = a.step;
@@ -163,7 +173,7 @@ OF_GLOBAL void OF_BOUNDS(256, 1) mt_begin_kernel(MtBeginArgs a) {
             t = *a.applied + 1;
             if (finite) *a.applied = t;
         }
-        float coef = a.max_norm > 0.f ? a.max_norm / (norm + 1e-6f) : 1.0f;
+        float coef = a.max_norm > 0.f ? 1.0f / (norm + 1e-6f) * a.max_norm : 1.0f;
         if (!(coef < 1.0f)) coef = 1.0f;
         a.out->coef = finite ? coef : -1.0f;
         a.out->t = t;
@@ -192,17 +202,18 @@ OF_DEV float mt_round_random(float q, unsigned u) {
 struct MtHyper {
     float coef, step_size, inv_sqrt_bc2, decay, beta1, omb1, beta2, omb2, eps;
 };
-// r receives the square root of the second moment
+// r receives the square root of the second moment.  Moments, root and everything that 8-bit codes are made of take one IEEE rounding per
+// written operation, in this order: where a value lies between two codes then does not depend on how the compiler joins operations.
+// The parameter's update goes into no later step: a 1-ulp reciprocal there (2e-7 of an update) saves its division.
 OF_DEV void mt_update(const MtHyper& h, f32x4& p, f32x4 g, f32x4& m, f32x4& v, f32x4& r) {
+#pragma clang fp contract(off)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float ge = h.coef * g[e];
-        m[e] = h.beta1 * m[e] + h.omb1 * ge;
-        v[e] = h.beta2 * v[e] + h.omb2 * ge * ge;
-        // 1-ulp reciprocal and square root: 2e-7 of an update that is itself a thousandth of the parameter (the IEEE forms are ~25
-        // instructions an element more, and 8-bit states are bound by instructions, not by memory)
-        r[e] = of_sqrt(v[e]);
-        p[e] = h.decay * p[e] - h.step_size * (m[e] * of_rcp(r[e] * h.inv_sqrt_bc2 + h.eps));
+        const float ge = g[e] * h.coef;
+        m[e] = m[e] * h.beta1 + ge * h.omb1;
+        v[e] = v[e] * h.beta2 + ge * h.omb2 * ge;
+        r[e] = sqrtf(v[e]);
+        p[e] = p[e] * h.decay - h.step_size * (m[e] * of_rcp(r[e] * h.inv_sqrt_bc2 + h.eps));
     }
 }
 
@@ -270,7 +281,7 @@ OF_GLOBAL void OF_BOUNDS(256, 4) mt_adamw_kernel(MtArgs a) {
             }
             tm = of_wave_max(tm);
             tr = of_wave_max(tr);
-            const float im = 448.0f / of_max(tm, 1e-30f), ir = 448.0f / of_max(tr, 1e-30f);          // (IEEE: once a block)
+            const float im = 1.0f / of_max(tm, 1e-30f) * 448.0f, ir = 1.0f / of_max(tr, 1e-30f) * 448.0f;          // (IEEE: once a block)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 m[u][e] = of_max(of_min(m[u][e] * im, 448.0f), -448.0f);
@@ -279,8 +290,8 @@ OF_GLOBAL void OF_BOUNDS(256, 4) mt_adamw_kernel(MtArgs a) {
             mt_store_codes(t.m, vec, i, n, of_f32_to_fp8x4(m[u]));
             mt_store_codes(t.v, vec, i, n, of_f32_to_fp8x4(r));
             if (lane == 0 && i < n) {
-                t.ms[i / BLOCK] = tm / 448.0f;
-                t.vs[i / BLOCK] = tr / 448.0f;
+                t.ms[i / BLOCK] = tm * (1.0f / 448.0f);
+                t.vs[i / BLOCK] = tr * (1.0f / 448.0f);
             }
         }
     }
@@ -290,7 +301,7 @@ int mt_launches(int n, int per) { return (n + per - 1) / per; }
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 }  // namespace
 
-extern "C" size_t of_adamw_multi_workspace_bytes(int n) { return n > 0 ? up256(sizeof(MtStep)) + (size_t)mt_launches(n, MT_NORM_MAX) * MT_PARTS * sizeof(float) : 0; }
+extern "C" size_t of_adamw_multi_workspace_bytes(int n) { return n > 0 ? up256(sizeof(MtStep)) + (size_t)mt_launches(n, MT_NORM_MAX) * MT_PARTS * sizeof(double) : 0; }
 
 extern "C" int of_adamw_multi(const OfAdamwTensor* tensors, int n, int bits, double beta1, double beta2, double eps, double max_norm, int step, int* applied_steps,
                               float* sumsq, void* workspace, size_t workspace_bytes, void* stream) {
@@ -307,7 +318,7 @@ extern "C" int of_adamw_multi(const OfAdamwTensor* tensors, int n, int bits, dou
     }
     of_stream_t s = (of_stream_t)stream;
     MtStep* st = (MtStep*)workspace;
-    float* parts = (float*)((char*)workspace + up256(sizeof(MtStep)));
+    double* parts = (double*)((char*)workspace + up256(sizeof(MtStep)));
     const int launches = mt_launches(n, MT_MAX), norms = mt_launches(n, MT_NORM_MAX);
     auto chunks = [](long elements, int chunk) { return (elements + chunk - 1) / chunk; };
     auto pack = [&](int l, MtArgs& a) {
@@ -346,11 +357,11 @@ extern "C" int of_adamw_multi(const OfAdamwTensor* tensors, int n, int bits, dou
             a.chunk_end[a.n++] = (int)end;
         }
         a.parts = parts + (size_t)l * MT_PARTS;
-        rc = of_launch(mt_sumsq_kernel, of_dim3{MT_PARTS, 1, 1}, 256, 4 * sizeof(float), s, a);
+        rc = of_launch(mt_sumsq_kernel, of_dim3{MT_PARTS, 1, 1}, 256, 256 * sizeof(double), s, a);
     }
     if (rc) return rc;
     const MtBeginArgs b{parts, (long)norms * MT_PARTS, (float)max_norm, beta1, beta2, step, applied_steps, st, sumsq};
-    rc = of_launch(mt_begin_kernel, of_dim3{1, 1, 1}, 256, 4 * sizeof(float), s, b);
+    rc = of_launch(mt_begin_kernel, of_dim3{1, 1, 1}, 256, 256 * sizeof(double), s, b);
     // last tensors first: the norm's launch read their gradients last, up to 256 MB of them are still in the Infinity Cache
     for (int l = launches - 1; l >= 0 && !rc; --l) {
         MtArgs a;

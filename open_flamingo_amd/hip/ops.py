@@ -514,12 +514,15 @@ class Ops:
 
     def embedding_bwd(self, ids, dy, dw, scale=1.0, padding_idx=-1):
         """dw[v] = scale * sum of dy[i] over ids[i] == v, every row written; positions with padding_idx or an id outside dw add nothing."""
-        assert ids.dtype == torch.int64 and ids.dim() == 1 and ids.is_contiguous() and dy.dtype == dw.dtype
-        assert dy.shape == (ids.numel(), dw.shape[1]) and dy.stride(1) == 1 and dw.stride(1) == 1
         n, (vocab, d) = ids.numel(), dw.shape
+        assert ids.dtype is torch.int64 and ids.dim() == 1 and ids.is_contiguous() and dy.dtype is dw.dtype and dy.shape == (n, d)
+        (ldy, cy), (ldw, cw) = dy.stride(), dw.stride()
+        assert cy == 1 and cw == 1
         ws = torch.empty(self.lib.of_embedding_bwd_workspace_bytes(n, vocab, d), dtype=torch.uint8, device=dw.device)
-        self._chk(self.lib.of_embedding_bwd(ids.data_ptr(), n, dy.data_ptr(), _is_f32(dy), max(dy.stride(0), d), vocab, d, scale, padding_idx,
-                                            dw.data_ptr(), max(dw.stride(0), d), ws.data_ptr(), ws.numel(), self._stream()), "of_embedding_bwd")
+        rc = self.lib.of_embedding_bwd(ids.data_ptr(), n, dy.data_ptr(), _is_f32(dy), max(ldy, d), vocab, d, scale, padding_idx,
+                                       dw.data_ptr(), max(ldw, d), ws.data_ptr(), ws.numel(), self._stream_fn())
+        if rc:
+            self._chk(rc, "of_embedding_bwd")
 
     # ------------------------------------------------------------------ AdamW over many tensors
     def adamw_multi(self, tensors, sumsq, *, bits, betas=(0.9, 0.999), eps=1e-8, max_norm=0.0, step=0, applied=None):

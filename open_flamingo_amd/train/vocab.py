@@ -6,7 +6,6 @@ through them.  They stand beside ``towers.use_libofhip_lm_loss``, which computes
 ``sparse_rows``, which trains two rows of a frozen table.  GPU tensors only, like everything that runs on libofhip.
 """
 import types
-from contextlib import nullcontext
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -27,10 +26,22 @@ def _rows16(t):
     return t.contiguous() if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _on(t):
-    """Context in which libofhip launches on ``t``'s device (nothing to do where it is the current one)."""
+def _elsewhere(t):
+    """a context for launches on ``t``'s device, or None where that is the current one (nothing to enter: host time of small calls)"""
     at = t.get_device()
-    return nullcontext() if at < 0 or at == torch.cuda.current_device() else torch.cuda.device(at)
+    return None if at < 0 or at == torch.cuda.current_device() else torch.cuda.device(at)
+
+
+def _backward(run, ctx, g):
+    """``run(ctx, g)`` on g's device.  Under create_graph the result is marked as differentiable once; without it there is no graph to mark,
+    and the marking's host time (as long as a small call's kernels) is left out."""
+    if torch.is_grad_enabled():
+        run = once_differentiable(run)
+    other = _elsewhere(g)
+    if other is None:
+        return run(ctx, g)
+    with other:
+        return run(ctx, g)
 
 
 def _linear_ce(hidden, table, labels, kw, ops, need):
@@ -52,13 +63,17 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        return _backward(_LinearCrossEntropy.run_backward, ctx, g)
+
+    @staticmethod
+    def run_backward(ctx, g):
         x, w, labels, state = ctx.saved_tensors
+        if g.dtype is not F32 or not g.is_contiguous():
+            g = g.to(F32).contiguous()
         dx = torch.empty(x.shape, dtype=BF16, device=x.device) if ctx.need[0] else None
         dw = torch.empty(w.shape, dtype=BF16, device=w.device) if ctx.need[1] else None
-        with _on(x):
-            ctx.ops.linear_ce_bwd(x, w, labels, state, g.to(F32).contiguous(), dx, dw, **ctx.kw)
+        ctx.ops.linear_ce_bwd(x, w, labels, state, g, dx, dw, **ctx.kw)
         return dx, dw, None, None, None
 
 
@@ -98,32 +113,41 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
         zero = (hidden.sum() + table[:0].sum()).to(F32)
         return zero.new_zeros(labels.shape) if reduction == "none" else zero / 0.0 if reduction == "mean" else zero
     kw = dict(ignore_index=int(ignore_index), logit_scale=float(logit_scale), reduction=_REDUCTION[reduction], piece=int(piece))
-    with _on(x):
+
+    def go():
         if torch.is_grad_enabled() and (x.requires_grad or table.requires_grad):
-            out = _LinearCrossEntropy.apply(x, table, y, kw, ops)
-        else:
-            out = _linear_ce(x, table, y, kw, ops, (False, False))[0]
+            return _LinearCrossEntropy.apply(x, table, y, kw, ops)
+        return _linear_ce(x, table, y, kw, ops, (False, False))[0]
+
+    other = _elsewhere(x)
+    if other is None:
+        out = go()
+    else:
+        with other:
+            out = go()
     return out.view(labels.shape) if reduction == "none" else out
 
 
 class _EmbeddingLookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, padding_idx, ops):
-        out = torch.empty(ids.numel(), table.shape[1], dtype=table.dtype, device=table.device)
+        out = table.new_empty((ids.shape[0], table.shape[1]))
         ops.embedding_fwd(ids, table, out, scale)
         ctx.save_for_backward(ids)
         ctx.shape, ctx.scale, ctx.padding_idx, ctx.ops = table.shape, scale, padding_idx, ops
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        return _backward(_EmbeddingLookup.run_backward, ctx, g)
+
+    @staticmethod
+    def run_backward(ctx, g):
         (ids,) = ctx.saved_tensors
-        if g.stride(-1) != 1:
+        if g.stride(1) != 1 or g.stride(0) < g.shape[1]:
             g = g.contiguous()
-        dw = torch.empty(ctx.shape, dtype=g.dtype, device=g.device)
-        with _on(g):
-            ctx.ops.embedding_bwd(ids, g, dw, ctx.scale, ctx.padding_idx)
+        dw = g.new_empty(ctx.shape)
+        ctx.ops.embedding_bwd(ids, g, dw, ctx.scale, ctx.padding_idx)
         return None, dw, None, None, None
 
 
@@ -153,12 +177,20 @@ def embedding_lookup(ids, table, *, scale=1.0, padding_idx=None, ops=None):
     if n == 0:
         return table[:0].reshape(*ids.shape, d) * scale
     t = table if table.stride(1) == 1 and table.stride(0) >= d else table.contiguous()
-    with _on(t):
+
+    def go():
         if t.requires_grad and torch.is_grad_enabled():
-            out = _EmbeddingLookup.apply(flat, t, float(scale), -1 if padding_idx is None else padding_idx, ops)
-        else:
-            out = t.new_empty((n, d))
-            ops.embedding_fwd(flat, t, out, scale)
+            return _EmbeddingLookup.apply(flat, t, float(scale), -1 if padding_idx is None else padding_idx, ops)
+        out = t.new_empty((n, d))
+        ops.embedding_fwd(flat, t, out, scale)
+        return out
+
+    other = _elsewhere(t)
+    if other is None:
+        out = go()
+    else:
+        with other:
+            out = go()
     return out if ids.dim() == 1 else out.view(*ids.shape, d)
 
 
