@@ -424,6 +424,70 @@ OF_GLOBAL void OF_BOUNDS(VEC_THREADS, 4) emb_join_kernel(EmbArgs a) {
     emb_store<F32, VEC>(a.dw, (size_t)cur * a.lddw + col, s, a.scale);
 }
 
+// At most 64 positions: every wave holds all ids, one a lane, and the ballot of the lanes that hold a row's id says which rows of dy make
+// it up, in ascending order.  One launch in place of sort, sum and join, and no row is written twice.  All positions on one row cost a
+// workgroup 64 rows of dy, AHEAD in flight.
+constexpr int FEW = 64;
+template <bool F32, bool VEC>
+OF_DEV void emb_few_sum(const EmbArgs& a, unsigned long long who, int col, float (&s)[8]) {
+    while (who) {
+        u32x4 x[AHEAD];
+        int many = 0;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (!who) break;
+            x[u] = emb_raw<F32, VEC>(a.dy, (size_t)__builtin_ctzll(who) * a.lddy + col);
+            who &= who - 1;
+            many = u + 1;
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (u < many) emb_add<F32, VEC>(x[u], s);
+    }
+}
+// any strides and widths: a row of the table per workgroup
+template <bool F32, bool VEC>
+OF_GLOBAL void OF_BOUNDS(VEC_THREADS, 4) emb_few_kernel(EmbArgs a) {
+    typedef EmbVec<F32, VEC> V;
+    const int tid = of_tid(), lane = tid & 63;
+    const int key = lane < a.n ? (int)emb_key(a, lane) : a.vocab;
+    for (long r = of_bid_x(); r < a.vocab; r += of_gdim_x()) {
+        const unsigned long long who = of_ballot(key == r);
+        for (int col = tid * V::W; col < a.d; col += VEC_THREADS * V::W) {
+            float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            emb_few_sum<F32, VEC>(a, who, col, s);
+            emb_store<F32, VEC>(a.dw, (size_t)r * a.lddw + col, s, who ? a.scale : 0.f);
+        }
+    }
+}
+// The table without gaps, in whole vectors: one vector per thread, 4 KB per workgroup, whatever the rows' ends.  Almost every workgroup finds
+// no position in its rows and writes zeros, at the rate of a fill: 50434 x 2048 fp32 in 61 us (61 for the fill alone; 74 with 16 KB per
+// workgroup), 47771 x 4008 in 120 (112; 138 by sort and sum, 156 with a row of the table per workgroup, two of which share a cache line),
+// 3461 x 2560 in 9 (17 by sort and sum).
+template <bool F32>
+OF_GLOBAL void OF_BOUNDS(VEC_THREADS, 4) emb_few_flat_kernel(EmbArgs a) {
+    typedef EmbVec<F32, true> V;
+    const int tid = of_tid(), lane = tid & 63, per = a.d / V::W;
+    const int key = lane < a.n ? (int)emb_key(a, lane) : a.vocab;
+    const long total = (long)a.vocab * per, lo = (long)of_bid_x() * VEC_THREADS, hi = lo + VEC_THREADS < total ? lo + VEC_THREADS : total, i = lo + tid;
+    unsigned long long left = of_ballot(key < a.vocab && key >= lo / per && key <= (hi - 1) / per);
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    bool any = false;
+    if (left) {          // (no lane has left: all of them hold ids)
+        const int r = (int)(i / per), col = (int)(i - (long)r * per) * V::W;
+        while (left) {
+            const int k = (int)of_readlane((unsigned)key, __builtin_ctzll(left));
+            const unsigned long long who = of_ballot(key == k);
+            left &= ~who;
+            if (r == k) {
+                emb_few_sum<F32, true>(a, who, col, s);
+                any = true;
+            }
+        }
+    }
+    if (i < hi) emb_store<F32, true>(a.dw, (size_t)i * V::W, s, any ? a.scale : 0.f);
+}
+
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 bool emb_small(long n, int vocab) { return n <= SMALL_MAX && vocab < (1 << 18); }
 int emb_passes(int vocab) {
@@ -441,6 +505,13 @@ bool emb_vec(const void* p, long ld, int d, int f32) { const int w = f32 ? 4 : 8
 
 template <bool F32, bool VEC>
 int emb_sums(const EmbArgs& a, of_stream_t s) {
+    if (a.n <= FEW) {
+        if constexpr (VEC) {
+            const long total = (long)a.vocab * (a.d / EmbVec<F32, VEC>::W);
+            if (a.lddw == a.d && total < (1l << 31)) return of_launch(emb_few_flat_kernel<F32>, of_dim3{(unsigned)((total + VEC_THREADS - 1) / VEC_THREADS), 1, 1}, VEC_THREADS, 0, s, a);
+        }
+        return of_launch(emb_few_kernel<F32, VEC>, of_dim3{(unsigned)(a.vocab < 16384 ? a.vocab : 16384), 1, 1}, VEC_THREADS, 0, s, a);
+    }
     const of_dim3 grid{(unsigned)a.chunks, (unsigned)((a.d + VEC_THREADS * EmbVec<F32, VEC>::W - 1) / (VEC_THREADS * EmbVec<F32, VEC>::W)), 1};
     const int rc = of_launch(emb_sum_kernel<F32, VEC>, grid, VEC_THREADS, 0, s, a);
     if (rc || a.chunks == 1) return rc;
@@ -459,14 +530,14 @@ extern "C" int of_embedding_fwd(const long long* ids, long n, const void* table,
 }
 
 extern "C" size_t of_embedding_bwd_workspace_bytes(long n, int vocab, int d) {
-    if (n <= 0 || vocab <= 0 || d <= 0) return 0;
+    if (n <= FEW || vocab <= 0 || d <= 0) return 0;
     const long nb = (n + TILE - 1) / TILE, chunks = (n + emb_chunk(n) - 1) / emb_chunk(n);
     return 4 * up256((size_t)n * 4) + up256((size_t)BINS * nb * 4) + up256((size_t)chunks * 2 * d * 4);
 }
 
 extern "C" int of_embedding_bwd(const long long* ids, long n, const void* dy, int f32, long lddy, int vocab, int d, float scale, long long padding_idx,
                                 void* dw, long lddw, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!ids || !dy || !dw || !workspace || n <= 0 || vocab <= 0 || d <= 0 || lddy < d || lddw < d || !emb_dtype_ok(f32)) return OF_E_ARG;
+    if (!ids || !dy || !dw || (!workspace && n > FEW) || n <= 0 || vocab <= 0 || d <= 0 || lddy < d || lddw < d || !emb_dtype_ok(f32)) return OF_E_ARG;
     if (n > (1l << 31) - 2 * TILE || vocab > (1 << 30)) return OF_E_SHAPE;
     if ((uintptr_t)workspace & 15) return OF_E_ALIGN;
     if (workspace_bytes < of_embedding_bwd_workspace_bytes(n, vocab, d)) return OF_E_WORKSPACE;
@@ -475,51 +546,53 @@ extern "C" int of_embedding_bwd(const long long* ids, long n, const void* dy, in
     a.ids = ids; a.n = n; a.vocab = vocab; a.d = d; a.padding_idx = padding_idx; a.f32 = f32; a.scale = scale;
     a.dy = dy; a.lddy = lddy; a.dw = dw; a.lddw = lddw;
     a.vec = emb_vec(dy, lddy, d, f32) && emb_vec(dw, lddw, d, f32);
-    char* ws = (char*)workspace;
-    auto take = [&](size_t bytes) {
-        char* p = ws;
-        ws += up256(bytes);
-        return p;
-    };
-    unsigned* key[2];
-    unsigned* pos[2];
-    for (int i = 0; i < 2; ++i) {
-        key[i] = (unsigned*)take((size_t)n * 4);
-        pos[i] = (unsigned*)take((size_t)n * 4);
-    }
-    a.nb = (int)((n + TILE - 1) / TILE);
-    a.hist = (int*)take((size_t)BINS * a.nb * 4);
-    a.chunk = emb_chunk(n);
-    a.chunks = (n + a.chunk - 1) / a.chunk;
-    a.part = (float*)take((size_t)a.chunks * 2 * d * 4);
-    a.passes = emb_passes(vocab);
-    const int fill = vocab < 2048 ? vocab : 2048;
-    int rc, in = 0;
-    if (emb_small(n, vocab)) {
-        a.key_out = key[0]; a.pos_out = pos[0];
-        a.cap = (int)(n + 63) / 64 * 64;
-        const size_t lds = 2 * (size_t)a.cap * 4 + SMALL_WAVES * BINS * 2 + BINS * 4;
-        // 256 workgroups sweep the table in windows of 4 MB: 766 MB cleared beside a sort of 39 positions takes 138 us in all; 255, 511
-        // and 1022 of them, whose windows do not end at a power of two, take 166, 155 and 170, 512 (two to a compute unit) 159
-        rc = of_launch(emb_sort_small_kernel, of_dim3{(unsigned)(1 + (fill < 256 ? fill : 256)), 1, 1}, SMALL_THREADS, lds, s, a);
-        if (rc) return rc;
-    } else {
-        for (int p = 0; p < a.passes; ++p) {
-            const int out = p & 1;
-            in = out ^ 1;
-            a.key_in = key[in]; a.pos_in = pos[in]; a.key_out = key[out]; a.pos_out = pos[out];
-            a.shift = p * RB;
-            a.from_ids = p == 0;
-            rc = of_launch(emb_count_kernel, of_dim3{(unsigned)(a.nb + (p == 0 ? fill : 0)), 1, 1}, TILE_THREADS, BINS * sizeof(int), s, a);
-            if (rc) return rc;
-            rc = of_launch(emb_scan_kernel, of_dim3{1, 1, 1}, BINS, BINS * sizeof(int), s, a);
-            if (rc) return rc;
-            rc = of_launch(emb_place_kernel, of_dim3{(unsigned)a.nb, 1, 1}, TILE_THREADS, (TILE_WAVES + 1) * BINS * sizeof(int), s, a);
-            if (rc) return rc;
-            in = out;
+    if (n > FEW) {
+        char* ws = (char*)workspace;
+        auto take = [&](size_t bytes) {
+            char* p = ws;
+            ws += up256(bytes);
+            return p;
+        };
+        unsigned* key[2];
+        unsigned* pos[2];
+        for (int i = 0; i < 2; ++i) {
+            key[i] = (unsigned*)take((size_t)n * 4);
+            pos[i] = (unsigned*)take((size_t)n * 4);
         }
+        a.nb = (int)((n + TILE - 1) / TILE);
+        a.hist = (int*)take((size_t)BINS * a.nb * 4);
+        a.chunk = emb_chunk(n);
+        a.chunks = (n + a.chunk - 1) / a.chunk;
+        a.part = (float*)take((size_t)a.chunks * 2 * d * 4);
+        a.passes = emb_passes(vocab);
+        const int fill = vocab < 2048 ? vocab : 2048;
+        int rc, in = 0;
+        if (emb_small(n, vocab)) {
+            a.key_out = key[0]; a.pos_out = pos[0];
+            a.cap = (int)(n + 63) / 64 * 64;
+            const size_t lds = 2 * (size_t)a.cap * 4 + SMALL_WAVES * BINS * 2 + BINS * 4;
+            // 256 workgroups sweep the table in windows of 4 MB: 766 MB cleared beside a sort of 39 positions takes 138 us in all; 255, 511
+            // and 1022 of them, whose windows do not end at a power of two, take 166, 155 and 170, 512 (two to a compute unit) 159
+            rc = of_launch(emb_sort_small_kernel, of_dim3{(unsigned)(1 + (fill < 256 ? fill : 256)), 1, 1}, SMALL_THREADS, lds, s, a);
+            if (rc) return rc;
+        } else {
+            for (int p = 0; p < a.passes; ++p) {
+                const int out = p & 1;
+                in = out ^ 1;
+                a.key_in = key[in]; a.pos_in = pos[in]; a.key_out = key[out]; a.pos_out = pos[out];
+                a.shift = p * RB;
+                a.from_ids = p == 0;
+                rc = of_launch(emb_count_kernel, of_dim3{(unsigned)(a.nb + (p == 0 ? fill : 0)), 1, 1}, TILE_THREADS, BINS * sizeof(int), s, a);
+                if (rc) return rc;
+                rc = of_launch(emb_scan_kernel, of_dim3{1, 1, 1}, BINS, BINS * sizeof(int), s, a);
+                if (rc) return rc;
+                rc = of_launch(emb_place_kernel, of_dim3{(unsigned)a.nb, 1, 1}, TILE_THREADS, (TILE_WAVES + 1) * BINS * sizeof(int), s, a);
+                if (rc) return rc;
+                in = out;
+            }
+        }
+        a.key = key[in]; a.pos = pos[in];
     }
-    a.key = key[in]; a.pos = pos[in];
     if (f32) return a.vec ? emb_sums<true, true>(a, s) : emb_sums<true, false>(a, s);
     return a.vec ? emb_sums<false, true>(a, s) : emb_sums<false, false>(a, s);
 }

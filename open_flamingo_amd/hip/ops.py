@@ -518,9 +518,10 @@ class Ops:
         assert ids.dtype is torch.int64 and ids.dim() == 1 and ids.is_contiguous() and dy.dtype is dw.dtype and dy.shape == (n, d)
         (ldy, cy), (ldw, cw) = dy.stride(), dw.stride()
         assert cy == 1 and cw == 1
-        ws = torch.empty(self.lib.of_embedding_bwd_workspace_bytes(n, vocab, d), dtype=torch.uint8, device=dw.device)
+        size = self.lib.of_embedding_bwd_workspace_bytes(n, vocab, d)
+        ws = torch.empty(size, dtype=torch.uint8, device=dw.device) if size else None
         rc = self.lib.of_embedding_bwd(ids.data_ptr(), n, dy.data_ptr(), _is_f32(dy), max(ldy, d), vocab, d, scale, padding_idx,
-                                       dw.data_ptr(), max(ldw, d), ws.data_ptr(), ws.numel(), self._stream_fn())
+                                       dw.data_ptr(), max(ldw, d), _p(ws), size, self._stream_fn())
         if rc:
             self._chk(rc, "of_embedding_bwd")
 

@@ -18,6 +18,10 @@ def run(ids, table, dy, **kw):
     (1, 1, 1, torch.float32, 1.0, None, "uniform"),
     (1, 8, 5, torch.bfloat16, 1.0, None, "uniform"),
     (40, 20, 7, torch.float32, 0.5, 3, "uniform"),           # every token crosses a chunk
+    (64, 8, 9, torch.float32, 1.0, None, "one"),             # 64: the longest without a sort
+    (64, 24, 40, torch.bfloat16, -2.0, 1, "bad"),
+    (63, 7, 5, torch.bfloat16, 1.0, None, "uniform"),
+    (65, 8, 5, torch.float32, 1.0, None, "one"),
     (300, 8, 50, torch.bfloat16, 45.25, -1, "skew"),
     (333, 12, 9, torch.float32, 1.0, None, "one"),           # one token over all chunks
     (333, 7, 9, torch.bfloat16, 2.0, None, "two"),           # columns that are no whole vectors

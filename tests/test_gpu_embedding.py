@@ -41,3 +41,28 @@ def test_the_same_bits_every_time():
     first = run(ids, table, dy)[1]
     for _ in range(5):
         assert torch.equal(run(ids, table, dy)[1], first)
+
+
+@pytest.mark.parametrize("n", [1, 64])
+def test_few_positions_of_a_wide_table(n):
+    R.emb_check(lambda ids, t, dy: run(ids, t, dy, scale=0.5, padding_idx=3), n, 2560, 3461, torch.float32, 0.5, 3, "bad", device="cuda")
+
+
+@pytest.mark.parametrize("n", [40, 300])
+def test_offsets_behind_32_bits(n):
+    vocab, d = 530001, 4096          # 2.2e9 elements, 4.3 GB
+    g = torch.Generator().manual_seed(0)
+    ids = torch.randint(0, vocab, (n,), generator=g).cuda()
+    ids[:4] = torch.tensor([vocab - 1, 0, vocab - 2, vocab - 1], device="cuda")
+    table = torch.empty(vocab, d, dtype=torch.bfloat16, device="cuda")
+    table[:] = torch.arange(d, device="cuda") % 64
+    table[:, 0] = (torch.arange(vocab, device="cuda") // 256).to(torch.bfloat16)
+    table[:, 1] = (torch.arange(vocab, device="cuda") % 256).to(torch.bfloat16)
+    dy = torch.randint(-8, 9, (n, d), generator=g).to(torch.bfloat16).cuda()          # sums of small whole numbers: exact
+    y, dt = run(ids, table, dy)
+    assert torch.equal(y, table[ids])
+    rows = ids.unique()
+    want = torch.zeros(rows.numel(), d, device="cuda").index_add_(0, torch.searchsorted(rows, ids), dy.float())
+    assert torch.equal(dt[rows].float(), want)
+    dt[rows] = 0
+    assert not dt.view(torch.int64).any()
