@@ -162,6 +162,13 @@ OF_DEV void xf_rows32_times_packed(const bf16_t* pk, const char* img, int wave, 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
+// a square rounded by itself (the sums of squares of both LayerNorms): an fma in its place depends on how the compiler pairs operations, and
+// where a gate's gradient is a small difference of large sums one ulp of the variance shows in its third digit
+OF_DEV float xf_square(float x) {
+#pragma clang fp contract(off)
+    return x * x;
+}
+
 template <int D>
 OF_GLOBAL void OF_BOUNDS(512, 2) of_xattn_fused_fwd_kernel(OfXattnFusedArgs p) {
     constexpr int CPL = (D + 511) / 512;        // 8-column chunks per lane of a row (wave per row)
@@ -264,7 +271,7 @@ OF_GLOBAL void OF_BOUNDS(512, 2) of_xattn_fused_fwd_kernel(OfXattnFusedArgs p) {
             for (int j = 0; j < CPL; ++j)
                 if (lo + j * 512 < (unsigned)D) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sq += (v[i][j][e] - mean) * (v[i][j][e] - mean);
+                    for (int e = 0; e < 8; ++e) sq += xf_square(v[i][j][e] - mean);
                 }
             const float rstd = of_rsqrt(of_wave_sum(sq) * inv_dim + 1e-5f);
             if (lane == 0 && p.stats) {
@@ -540,7 +547,7 @@ OF_GLOBAL void OF_BOUNDS(512, 2) of_xattn_fused_fwd_kernel(OfXattnFusedArgs p) {
 #pragma unroll
         for (int t = 0; t < NTO; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sq += (yacc[mt][t][r] - mean[mt]) * (yacc[mt][t][r] - mean[mt]);
+            for (int r = 0; r < 4; ++r) sq += xf_square(yacc[mt][t][r] - mean[mt]);
         sq = of_rows_sum(sq);
         if (g == 0) red[256 + wave * 32 + mt * 16 + i16] = sq;
     }
