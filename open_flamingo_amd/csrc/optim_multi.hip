@@ -3,7 +3,8 @@
 //   p  = p (1 - lr wd) - lr / (1 - b1^t)  m / (sqrt(v / (1 - b2^t)) + eps)
 // An element costs 28 bytes of traffic with fp32 moments and gradients, 16 with 8-bit moments, and 4 more for the norm.  One launch takes
 // up to 48 tensors (their pointers travel in the kernel arguments: nothing to keep in step on the device, safe to capture); a
-// workgroup takes 4096 elements of one tensor.
+// workgroup takes 4096 elements of one tensor.  Measured (160 tensors, 120 million elements, fp32 gradients, with the clip): 760 us with fp32
+// moments = 3.84 GB at 5.05 TB/s, a large copy's rate (update 620, norm 125 us); 492 us with 8-bit moments = 2.40 GB at 4.9 TB/s.
 //
 // 8-bit moments: e4m3 codes with one fp32 scale (largest magnitude / 448) per 256 consecutive elements of a tensor.
 //   * The first moment is rounded to the nearest code: it moves by a tenth of its distance to g' every step, more than half a code.
