@@ -466,8 +466,9 @@ class Ops:
         return a
 
     def _linear_ce_workspace(self, a, backward, device):
-        ws = torch.empty(self.lib.of_linear_ce_workspace_bytes(a, backward), dtype=torch.uint8, device=device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        size = self.lib.of_linear_ce_workspace_bytes(a, backward)
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), size
         return ws
 
     def linear_ce_fwd(self, x, w, labels, loss_rows, loss=None, *, ignore_index=-100, logit_scale=1.0, reduction=abi.CE_MEAN, piece=0, need=(False, False)):
@@ -479,8 +480,9 @@ class Ops:
         a.loss_rows, a.loss = loss_rows.data_ptr(), _p(loss)
         state = None
         if need[0] or need[1] or not self.lib.of_linear_ce_stateless(a.rows, a.d):
-            state = torch.empty(self.lib.of_linear_ce_state_bytes(a), dtype=torch.uint8, device=x.device)
-            a.state, a.state_bytes = state.data_ptr(), state.numel()
+            size = self.lib.of_linear_ce_state_bytes(a)
+            state = torch.empty(size, dtype=torch.uint8, device=x.device)
+            a.state, a.state_bytes = state.data_ptr(), size
         ws = self._linear_ce_workspace(a, 0, x.device)          # noqa: F841 (alive until the launches are enqueued)
         self._chk(self.lib.of_linear_ce_fwd(a, self._stream()), "of_linear_ce_fwd")
         return state

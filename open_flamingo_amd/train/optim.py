@@ -413,7 +413,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=0, lr=1e-3, betas=(
     device, none overlapping another.  lr, weight_decay: one value, or one per tensor.  max_norm <= 0: no clipping.
 
     step: 1-based count of this update; ``applied``, a device int32 counter, replaces it, and counts the updates that were applied.  A
-    gradient norm that is not finite leaves everything untouched (no host synchronisation).  Returns the squared norm (1, fp32)."""
+    gradient norm that is not finite leaves everything untouched (no host synchronisation).  May be captured into a graph: a replay keeps
+    the tensors' addresses, lr, weight_decay and step (give ``applied`` there).  Returns the squared norm (1, fp32)."""
     n = len(params)
     coded = exp_avg_scales is not None or exp_avg_sq_scales is not None
     lists = [grads, exp_avgs, exp_avg_sqs] + ([exp_avg_scales or (), exp_avg_sq_scales or ()] if coded else [])
@@ -465,6 +466,10 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=0, lr=1e-3, betas=(
     return sumsq
 
 
+def _capturing():
+    return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+
+
 class MultiTensorAdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` for fp32 parameters through ``adamw_step``: every ``step()`` is one call over all parameters that have a gradient,
     whatever they are (a fully trained vocabulary table included, which ``FlatAdamW`` refuses), with ``clip_grad_norm_(max_norm)`` in it and no
@@ -489,6 +494,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     def _state_of(self, p):
         st = self.state[p]
         if not st:
+            if _capturing():          # a replay would clear them again
+                raise RuntimeError("MultiTensorAdamW makes its moments at a parameter's first step: take one before capturing step()")
             if self.state_bits == 32:
                 st["exp_avg"], st["exp_avg_sq"] = torch.zeros_like(p), torch.zeros_like(p)
             else:

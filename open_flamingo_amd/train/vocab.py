@@ -47,8 +47,8 @@ def _backward(run, ctx, g):
 def _linear_ce(hidden, table, labels, kw, ops, need):
     """(loss, what a backward needs)"""
     x, w = _rows16(hidden), _rows16(table)
-    loss_rows = torch.empty(x.shape[0], dtype=F32, device=x.device)
-    loss = torch.empty((), dtype=F32, device=x.device) if kw["reduction"] != abi.CE_NONE else None
+    loss_rows = x.new_empty(x.shape[0], dtype=F32)
+    loss = x.new_empty((), dtype=F32) if kw["reduction"] != abi.CE_NONE else None
     state = ops.linear_ce_fwd(x, w, labels, loss_rows, loss, need=need, **kw)
     return loss_rows if loss is None else loss, (x, w, labels, state)
 
@@ -71,8 +71,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         x, w, labels, state = ctx.saved_tensors
         if g.dtype is not F32 or not g.is_contiguous():
             g = g.to(F32).contiguous()
-        dx = torch.empty(x.shape, dtype=BF16, device=x.device) if ctx.need[0] else None
-        dw = torch.empty(w.shape, dtype=BF16, device=w.device) if ctx.need[1] else None
+        dx = x.new_empty(x.shape) if ctx.need[0] else None
+        dw = w.new_empty(w.shape) if ctx.need[1] else None
         ctx.ops.linear_ce_bwd(x, w, labels, state, g, dx, dw, **ctx.kw)
         return dx, dw, None, None, None
 
@@ -88,44 +88,48 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
     holds a logits gradient of at a time (0: chosen, 128 MB of it)."""
     if reduction not in _REDUCTION:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {reduction!r}")
-    if hidden.shape[:-1] != labels.shape:
-        raise ValueError(f"labels {tuple(labels.shape)} do not fit hidden states {tuple(hidden.shape)}")
-    if table.dim() != 2 or table.shape[1] != hidden.shape[-1] or table.shape[0] == 0:
-        raise ValueError(f"table {tuple(table.shape)} does not fit hidden states {tuple(hidden.shape)}")
-    if (labels.numel() + 255) // 256 * 256 * ((hidden.shape[-1] + 63) // 64 * 64) >= 1 << 31:
-        raise ValueError(f"{labels.numel()} rows of {hidden.shape[-1]}: the hidden states of a call must stay below 2^31 elements; split the batch")
-    if hidden.shape[-1] % 8:
-        raise ValueError(f"the hidden size must be a multiple of 8, got {hidden.shape[-1]}")
-    if labels.dtype != torch.int64:
+    shape, d, n = hidden.shape, hidden.shape[-1], labels.numel()
+    if shape[:-1] != labels.shape:
+        raise ValueError(f"labels {tuple(labels.shape)} do not fit hidden states {tuple(shape)}")
+    if table.dim() != 2 or table.shape[1] != d or table.shape[0] == 0:
+        raise ValueError(f"table {tuple(table.shape)} does not fit hidden states {tuple(shape)}")
+    if (n + 255) // 256 * 256 * ((d + 63) // 64 * 64) >= 1 << 31:
+        raise ValueError(f"{n} rows of {d}: the hidden states of a call must stay below 2^31 elements; split the batch")
+    if d % 8:
+        raise ValueError(f"the hidden size must be a multiple of 8, got {d}")
+    if labels.dtype is not torch.int64:
         raise TypeError(f"labels must be int64, got {labels.dtype}")
     if piece < 0:
         raise ValueError("piece must not be negative")
     if not hidden.get_device() == table.get_device() == labels.get_device():
         raise ValueError(f"hidden, table and labels are on {hidden.device}, {table.device} and {labels.device}")
-    ops = _ops_for(hidden, ops, "linear_cross_entropy")
-    dev = hidden.device.type
-    if torch.is_autocast_enabled(dev) and torch.get_autocast_dtype(dev) == BF16:
-        hidden, table = hidden.to(BF16), table.to(BF16)
-    if hidden.dtype != BF16 or table.dtype != BF16:
-        raise TypeError(f"linear_cross_entropy takes bfloat16 operands (or runs under bf16 autocast), got {hidden.dtype} and {table.dtype}")
-    x, y = hidden.reshape(-1, hidden.shape[-1]), labels.reshape(-1).contiguous()
-    if x.shape[0] == 0:          # no rows: torch's values, zero gradients
+    if ops is None:
+        ops = _ops_for(hidden, ops, "linear_cross_entropy")
+    if hidden.dtype is not BF16 or table.dtype is not BF16:
+        dev = hidden.device.type
+        if torch.is_autocast_enabled(dev) and torch.get_autocast_dtype(dev) == BF16:
+            hidden, table = hidden.to(BF16), table.to(BF16)
+        if hidden.dtype is not BF16 or table.dtype is not BF16:
+            raise TypeError(f"linear_cross_entropy takes bfloat16 operands (or runs under bf16 autocast), got {hidden.dtype} and {table.dtype}")
+    x = hidden if len(shape) == 2 else hidden.reshape(-1, d)
+    y = labels if len(shape) == 2 and labels.is_contiguous() else labels.reshape(-1).contiguous()
+    if n == 0:          # no rows: torch's values, zero gradients
         zero = (hidden.sum() + table[:0].sum()).to(F32)
         return zero.new_zeros(labels.shape) if reduction == "none" else zero / 0.0 if reduction == "mean" else zero
     kw = dict(ignore_index=int(ignore_index), logit_scale=float(logit_scale), reduction=_REDUCTION[reduction], piece=int(piece))
-
-    def go():
-        if torch.is_grad_enabled() and (x.requires_grad or table.requires_grad):
-            return _LinearCrossEntropy.apply(x, table, y, kw, ops)
-        return _linear_ce(x, table, y, kw, ops, (False, False))[0]
-
     other = _elsewhere(x)
     if other is None:
-        out = go()
+        out = _run_linear_ce(x, table, y, kw, ops)
     else:
         with other:
-            out = go()
-    return out.view(labels.shape) if reduction == "none" else out
+            out = _run_linear_ce(x, table, y, kw, ops)
+    return out.view(labels.shape) if reduction == "none" and len(shape) != 2 else out
+
+
+def _run_linear_ce(x, table, y, kw, ops):
+    if (x.requires_grad or table.requires_grad) and torch.is_grad_enabled():
+        return _LinearCrossEntropy.apply(x, table, y, kw, ops)
+    return _linear_ce(x, table, y, kw, ops, (False, False))[0]
 
 
 class _EmbeddingLookup(torch.autograd.Function):
@@ -149,6 +153,14 @@ class _EmbeddingLookup(torch.autograd.Function):
         dw = g.new_empty(ctx.shape)
         ctx.ops.embedding_bwd(ids, g, dw, ctx.scale, ctx.padding_idx)
         return None, dw, None, None, None
+
+
+def _run_embedding(ids, t, scale, padding_idx, ops):
+    if t.requires_grad and torch.is_grad_enabled():
+        return _EmbeddingLookup.apply(ids, t, scale, padding_idx, ops)
+    out = t.new_empty((ids.shape[0], t.shape[1]))
+    ops.embedding_fwd(ids, t, out, scale)
+    return out
 
 
 def embedding_lookup(ids, table, *, scale=1.0, padding_idx=None, ops=None):
@@ -178,19 +190,13 @@ def embedding_lookup(ids, table, *, scale=1.0, padding_idx=None, ops=None):
         return table[:0].reshape(*ids.shape, d) * scale
     t = table if table.stride(1) == 1 and table.stride(0) >= d else table.contiguous()
 
-    def go():
-        if t.requires_grad and torch.is_grad_enabled():
-            return _EmbeddingLookup.apply(flat, t, float(scale), -1 if padding_idx is None else padding_idx, ops)
-        out = t.new_empty((n, d))
-        ops.embedding_fwd(flat, t, out, scale)
-        return out
-
+    pad = -1 if padding_idx is None else padding_idx
     other = _elsewhere(t)
     if other is None:
-        out = go()
+        out = _run_embedding(flat, t, float(scale), pad, ops)
     else:
         with other:
-            out = go()
+            out = _run_embedding(flat, t, float(scale), pad, ops)
     return out if ids.dim() == 1 else out.view(*ids.shape, d)
 
 
@@ -216,7 +222,7 @@ def _keeps_all(logits_to_keep):
 
 
 def _embedding_forward(self, ids):
-    if ids.dtype == torch.int64 and _runs_here(self.weight):
+    if ids.dtype == torch.int64 and self.weight.dtype in (F32, BF16) and _runs_here(self.weight):
         return embedding_lookup(ids, self.weight, padding_idx=self.padding_idx)
     return self._of_eager_forward(ids)
 
