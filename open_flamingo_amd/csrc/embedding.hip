@@ -4,7 +4,8 @@
 // The gradient has to read dy once (n x d) and to write the table once (vocabulary x d); torch scatters with atomics into a zeroed
 // table and rounds behind every addition where the table is bf16.  Here, without floating-point atomics:
 //   sort     (id, position) by id, stable: radix passes of 9 bits.  Up to 16384 positions ONE workgroup sorts in LDS while the
-//            others of the same launch clear the table; more positions take three launches a pass (counts, their scan, placement).
+//            others of the same launch clear the table; more positions take two launches a pass (counts, placement), from 2^22 + 1 on a
+//            third that adds the counts up.
 //            Ids that have no gradient (padding_idx, ids outside the table) sort behind all others.
 //   sum      a workgroup takes a chunk of the sorted list and 256 vectors of columns and walks the chunk with the running sum in
 //            registers.  A token whose positions lie inside the chunk is finished there; the two that cross its ends leave fp32
@@ -12,7 +13,7 @@
 //   join     the chunk in which a crossing token begins adds the partial rows of the chunks behind it, in order.
 // The same ids and gradients give the same bits on every run.
 // Measured: 8192 tokens of a 50435 x 2048 fp32 table, forward and gradient 134 us (lookup 38, sort beside the clearing of 413 MB 58, sums 32, join
-// 5; 614 MB); 32768 tokens, 4096 columns of bf16, skewed ids: 323 us (lookup 89, sort and clearing 108, sums 114, join 14).
+// 5; 614 MB); 32768 tokens, 4096 columns of bf16, skewed ids: 306 us (lookup 89, the rest 218).
 #include "gemm_common.h"
 
 namespace {
@@ -21,6 +22,8 @@ constexpr int RB = 9, BINS = 1 << RB;            // two passes up to a vocabular
 constexpr int SMALL_MAX = 16384;                 // positions one workgroup sorts in LDS
 constexpr int SMALL_THREADS = 1024;
 constexpr int TILE = 4096, TILE_THREADS = 512;   // positions per workgroup of a pass over more
+constexpr int SCAN_TILES = 1024;                 // up to this many tiles each adds their counts up for itself: a launch less per pass (32768
+                                                 // positions x 4096, gradient: 234 -> 218 us with 8 tiles; 1048576 x 64: 431 -> 380 with 256; 4000000: 1537 -> 1347)
 constexpr int VEC_THREADS = 256;
 
 struct EmbArgs {
@@ -100,11 +103,21 @@ OF_DEV unsigned long long emb_match(unsigned digit, bool live) {
 }
 OF_DEV int emb_below(unsigned long long m, int lane) { return __builtin_popcountll(m & ((1ull << lane) - 1)); }
 
+// running sums over the bins, in place; every thread of the workgroup calls it
+OF_DEV void emb_scan_bins(int* cum, int tid) {
+    for (int o = 1; o < BINS; o <<= 1) {
+        const int v = tid < BINS && tid >= o ? cum[tid - o] : 0;
+        of_sync();
+        if (tid < BINS) cum[tid] += v;
+        of_sync();
+    }
+}
+
 // Turns cnt[wave][digit] (how often each wave met each digit) into the place of the wave's first such element: in a tile of its own
 // (base = nullptr), or behind base[digit * stride].  The waves hold consecutive parts of the tile: the order stays.  LDS: cnt, cum[BINS];
 // every thread of the workgroup calls.
 template <class CNT>
-OF_DEV void emb_offsets(CNT* cnt, int* cum, int waves, int tid, const int* base, long stride) {
+OF_DEV void emb_offsets(CNT* cnt, int* cum, int waves, int tid, bool given, int at) {
     of_sync();
     int total = 0;
     if (tid < BINS) {
@@ -112,16 +125,8 @@ OF_DEV void emb_offsets(CNT* cnt, int* cum, int waves, int tid, const int* base,
         cum[tid] = total;
     }
     of_sync();
-    int at;
-    if (base) {
-        at = tid < BINS ? base[tid * stride] : 0;
-    } else {
-        for (int o = 1; o < BINS; o <<= 1) {
-            const int v = tid < BINS && tid >= o ? cum[tid - o] : 0;
-            of_sync();
-            if (tid < BINS) cum[tid] += v;
-            of_sync();
-        }
+    if (!given) {
+        emb_scan_bins(cum, tid);
         at = tid < BINS ? cum[tid] - total : 0;
     }
     if (tid < BINS)
@@ -184,7 +189,7 @@ OF_GLOBAL void OF_BOUNDS(SMALL_THREADS, 1) emb_sort_small_kernel(EmbArgs a) {
                 of_wave_sync();
             }
         }
-        emb_offsets(cnt, cum, SMALL_WAVES, tid, nullptr, 0);
+        emb_offsets(cnt, cum, SMALL_WAVES, tid, false, 0);
 #pragma unroll
         for (int it = 0; it < SMALL_ITERS; ++it) {
             if (it < iters) {
@@ -206,10 +211,10 @@ OF_GLOBAL void OF_BOUNDS(SMALL_THREADS, 1) emb_sort_small_kernel(EmbArgs a) {
     }
 }
 
-// ---- more positions: three launches a pass.  key / position i of the pass's input (the first pass reads the ids)
+// ---- more positions: two or three launches a pass.  key / position i of the pass's input (the first pass reads the ids)
 OF_DEV unsigned emb_in_key(const EmbArgs& a, long i) { return a.from_ids ? emb_key(a, i) : a.key_in[i]; }
 
-// counts of the digits of every tile: hist[digit][tile]; workgroups behind the tiles clear the table
+// counts of the digits of every tile: hist[tile][digit]; workgroups behind the tiles clear the table
 OF_GLOBAL void OF_BOUNDS(TILE_THREADS, 2) emb_count_kernel(EmbArgs a) {
     const int tid = of_tid();
     if (of_bid_x() >= a.nb) {
@@ -222,27 +227,22 @@ OF_GLOBAL void OF_BOUNDS(TILE_THREADS, 2) emb_count_kernel(EmbArgs a) {
     const long first = (long)of_bid_x() * TILE;
     for (long i = first + tid; i < first + TILE && i < a.n; i += TILE_THREADS) of_lds_count(cnt + ((emb_in_key(a, i) >> a.shift) & (BINS - 1)), 1);
     of_sync();
-    a.hist[(size_t)tid * a.nb + of_bid_x()] = cnt[tid];
+    a.hist[(size_t)of_bid_x() * BINS + tid] = cnt[tid];
 }
 // hist -> the place of every (digit, tile)'s first element; one workgroup, a thread per digit
 OF_GLOBAL void OF_BOUNDS(BINS, 1) emb_scan_kernel(EmbArgs a) {
     int* cum = (int*)of_smem();
     const int tid = of_tid();
-    int* mine = a.hist + (size_t)tid * a.nb;
+    int* mine = a.hist + tid;
     int total = 0;
-    for (int b = 0; b < a.nb; ++b) total += mine[b];
+    for (int b = 0; b < a.nb; ++b) total += mine[(size_t)b * BINS];
     cum[tid] = total;
     of_sync();
-    for (int o = 1; o < BINS; o <<= 1) {
-        const int v = tid >= o ? cum[tid - o] : 0;
-        of_sync();
-        cum[tid] += v;
-        of_sync();
-    }
+    emb_scan_bins(cum, tid);
     int at = cum[tid] - total;
     for (int b = 0; b < a.nb; ++b) {
-        const int c = mine[b];
-        mine[b] = at;
+        const int c = mine[(size_t)b * BINS];
+        mine[(size_t)b * BINS] = at;
         at += c;
     }
 }
@@ -254,6 +254,13 @@ OF_GLOBAL void OF_BOUNDS(TILE_THREADS, 2) emb_place_kernel(EmbArgs a) {
     int* mine = cnt + wave * BINS;
     for (int i = tid; i < TILE_WAVES * BINS; i += TILE_THREADS) cnt[i] = 0;
     of_sync();
+    int total = 0, earlier = 0;          // of digit `tid`: in all tiles, in those in front of this one
+    if (a.nb <= SCAN_TILES)
+        for (int b = 0; b < a.nb; ++b) {
+            const int c = a.hist[(size_t)b * BINS + tid];
+            total += c;
+            if (b < of_bid_x()) earlier += c;
+        }
     const long lo = (long)of_bid_x() * TILE + wave * TILE_ITERS * 64;
     int rank[TILE_ITERS];
     unsigned key[TILE_ITERS], pos[TILE_ITERS];
@@ -274,7 +281,16 @@ OF_GLOBAL void OF_BOUNDS(TILE_THREADS, 2) emb_place_kernel(EmbArgs a) {
         if (live && before == 0) mine[digit] += __builtin_popcountll(same);
         of_wave_sync();
     }
-    emb_offsets(cnt, cum, TILE_WAVES, tid, a.hist + of_bid_x(), (long)a.nb);
+    int at = 0;          // place of this tile's first element of digit `tid`
+    if (a.nb > SCAN_TILES) {
+        at = a.hist[(size_t)of_bid_x() * BINS + tid];
+    } else {
+        cum[tid] = total;
+        of_sync();
+        emb_scan_bins(cum, tid);
+        at = cum[tid] - total + earlier;
+    }
+    emb_offsets(cnt, cum, TILE_WAVES, tid, true, at);
 #pragma unroll
     for (int it = 0; it < TILE_ITERS; ++it) {
         if (lo + it * 64 + lane < a.n) {
@@ -497,9 +513,10 @@ int emb_passes(int vocab) {
     while ((vocab >> bits) != 0) ++bits;
     return (bits + RB - 1) / RB;
 }
-// Positions per chunk of the sums: enough chunks to fill the chip, few enough that joining one token that fills them all stays short
+// Positions per chunk of the sums: enough chunks to fill the chip, few enough that joining one token that fills them all stays short.  32768
+// positions of 4096 columns: 259 us in all with chunks of 8, 242 / 236 / 228 / 226 with 16 / 32 / 64 / 128; 2048 positions of 2048: 84, 84, 92, 109 with 8, 16, 64, 128
 int emb_chunk(long n) {
-    long c = n / 1024;
+    long c = n / 512 < 64 ? n / 512 : n / 1024 < 64 ? 64 : n / 1024;
     return (int)(c < 16 ? 16 : c > 4096 ? 4096 : (c + AHEAD - 1) / AHEAD * AHEAD);
 }
 int emb_dtype_ok(int f32) { return f32 == 0 || f32 == 1; }
@@ -586,7 +603,7 @@ extern "C" int of_embedding_bwd(const long long* ids, long n, const void* dy, in
                 a.from_ids = p == 0;
                 rc = of_launch(emb_count_kernel, of_dim3{(unsigned)(a.nb + (p == 0 ? fill : 0)), 1, 1}, TILE_THREADS, BINS * sizeof(int), s, a);
                 if (rc) return rc;
-                rc = of_launch(emb_scan_kernel, of_dim3{1, 1, 1}, BINS, BINS * sizeof(int), s, a);
+                if (a.nb > SCAN_TILES) rc = of_launch(emb_scan_kernel, of_dim3{1, 1, 1}, BINS, BINS * sizeof(int), s, a);
                 if (rc) return rc;
                 rc = of_launch(emb_place_kernel, of_dim3{(unsigned)a.nb, 1, 1}, TILE_THREADS, (TILE_WAVES + 1) * BINS * sizeof(int), s, a);
                 if (rc) return rc;

@@ -529,7 +529,7 @@ OF_DEV void of_gelu_both(float a, float& gelu, float& dgelu) {
     dgelu = cdf + a * 0.39894228040143268f * e;
 }
 // ---- the same for TWO elements per lane, written as two-element vectors -- the big-tile GEMM epilogues.  (The build keeps the packed
-// fp32 instructions off, csrc/build.py: every operation below is issued once per element.)  Round 4's tile phase probe showed the erf-GELU epilogues to be bound by VALU
+// fp32 instructions off, csrc/build.py: every operation below is issued once per element.)  A tile phase probe showed the erf-GELU epilogues to be bound by VALU
 // issue of the one wave a SIMD holds (~90 cycles per element through the scalar forms above, 9 of the 12.6 us a GELU
 // tile spends behind its K loop), and the quarter-rate transcendentals to be a third of that.
 //   forward (Phi only): Abramowitz-Stegun 7.1.28, erf(x) = 1 - (1 + a1 x + .. + a6 x^6)^-16, |error| <= 3e-7: ONE transcendental

@@ -54,7 +54,7 @@ def test_the_loss_stays_inside_its_buffers(guarded, rows, d, vocab, piece, table
     guarded.check()
 
 
-@pytest.mark.parametrize("n,d,vocab", [(1, 4, 3), (64, 5, 9), (65, 4, 9), (1000, 12, 70000), (20000, 2, 300), (17000, 1, 1)])
+@pytest.mark.parametrize("n,d,vocab", [(1, 4, 3), (64, 5, 9), (65, 4, 9), (1000, 12, 70000), (20000, 2, 300), (17000, 1, 1), (131073, 1, 300)])
 def test_the_lookup_stays_inside_its_buffers(guarded, n, d, vocab):
     ops = harness.emu_ops()
     ids = torch.randint(-1, vocab + 1, (n,), generator=torch.Generator().manual_seed(0))

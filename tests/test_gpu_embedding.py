@@ -29,6 +29,9 @@ def run(ids, table, dy, **kw):
     (70000, 40, 66000, torch.float32, 1.0, None, "uniform"),
     (100000, 8, 300000, torch.float32, 1.0, None, "skew"),
     (50001, 16, 11, torch.float32, 1.0, 4, "one"),
+    (131072, 8, 5000, torch.float32, 1.0, None, "skew"),
+    (4194305, 1, 600000, torch.float32, 1.0, None, "uniform"),          # the counts are added up by a launch of their own
+    (300000, 8, 700000, torch.bfloat16, 1.0, 5, "skew"),
 ])
 def test_lookup_and_gradient(n, d, vocab, dtype, scale, padding_idx, kind):
     R.emb_check(lambda ids, t, dy: run(ids, t, dy, scale=scale, padding_idx=padding_idx), n, d, vocab, dtype, scale, padding_idx, kind, device="cuda")
