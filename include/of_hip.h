@@ -418,7 +418,8 @@ int of_linear_ce_bwd(const OfLinearCeArgs* args, void* stream);
  *   of_embedding_fwd: y[i] = scale * table[ids[i]]; NaN in the rows of ids outside [0, vocab) (nothing is read for them)
  *   of_embedding_bwd: dw[v] = scale * sum over {i: ids[i] = v} dy[i], summed in fp32 in ascending i, EVERY row written (zeros without a
  *              token); positions whose id is padding_idx (-1: none is) or outside the table add nothing.  Deterministic: the positions are
- *              sorted by id, no floating-point atomics.  Workspace: of_embedding_bwd_workspace_bytes, 16-byte aligned. */
+ *              sorted by id, no floating-point atomics.  Workspace: of_embedding_bwd_workspace_bytes, 16-byte aligned (NULL where that is 0: up to
+ *              64 positions). */
 int of_embedding_fwd(const long long* ids, long n, const void* table, int f32, long ldt, int vocab, int d, float scale, void* y, long ldy,
                      void* stream);
 size_t of_embedding_bwd_workspace_bytes(long n, int vocab, int d);
