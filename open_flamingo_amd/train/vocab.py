@@ -8,6 +8,7 @@ through them.  They stand beside ``towers.use_libofhip_lm_loss``, which computes
 import types
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ..hip import abi
@@ -30,6 +31,17 @@ def _elsewhere(t):
     """a context for launches on ``t``'s device, or None where that is the current one (nothing to enter: host time of small calls)"""
     at = t.get_device()
     return None if at < 0 or at == torch.cuda.current_device() else torch.cuda.device(at)
+
+
+def _forward_mode():
+    """Tangents may be attached to the operands (forward-mode AD: inside a dual level, with gradients switched off as well)."""
+    return forward_ad._current_level >= 0
+
+
+def _needs_node(*tensors):
+    """The call has to be an autograd node: an operand wants a gradient, or may carry a tangent, which a bare launch would drop and the node
+    refuses (NotImplementedError: the operators have a backward only)."""
+    return _forward_mode() or (torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
 
 
 def _backward(run, ctx, g):
@@ -85,7 +97,7 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
     multiple of 8.  labels (...): int64, already shifted.  reduction "mean" (over the labels that count: NaN without any), "sum" or
     "none" (one fp32 loss per label, 0 where ignored).  A label outside the vocabulary that is not ``ignore_index`` makes the loss NaN and
     has no gradient.  Where the table has no gradient the forward prepares the hidden states' one from the same product.  Gradients come in bfloat16 for both operands, through fp32 sums; ``piece``: vocabulary rows the backward
-    holds a logits gradient of at a time (0: chosen, 128 MB of it)."""
+    holds a logits gradient of at a time (0: chosen, 128 MB of it).  Differentiable once, backward; forward-mode AD raises."""
     if reduction not in _REDUCTION:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {reduction!r}")
     shape, d, n = hidden.shape, hidden.shape[-1], labels.numel()
@@ -127,7 +139,7 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
 
 
 def _run_linear_ce(x, table, y, kw, ops):
-    if (x.requires_grad or table.requires_grad) and torch.is_grad_enabled():
+    if _needs_node(x, table):
         return _LinearCrossEntropy.apply(x, table, y, kw, ops)
     return _linear_ce(x, table, y, kw, ops, (False, False))[0]
 
@@ -156,7 +168,7 @@ class _EmbeddingLookup(torch.autograd.Function):
 
 
 def _run_embedding(ids, t, scale, padding_idx, ops):
-    if t.requires_grad and torch.is_grad_enabled():
+    if _needs_node(t):
         return _EmbeddingLookup.apply(ids, t, scale, padding_idx, ops)
     out = t.new_empty((ids.shape[0], t.shape[1]))
     ops.embedding_fwd(ids, t, out, scale)
@@ -168,7 +180,7 @@ def embedding_lookup(ids, table, *, scale=1.0, padding_idx=None, ops=None):
     fixed order (the same bits on every run) and rounded once.
 
     ids: int64 of any shape; an id outside the table gives a row of NaN and no gradient.  padding_idx (None: none; negative: counted
-    from the table's end): that row gets no gradient."""
+    from the table's end): that row gets no gradient.  Differentiable once, backward; forward-mode AD raises."""
     if table.dim() != 2 or 0 in table.shape:
         raise ValueError(f"table must be (vocabulary, d), got {tuple(table.shape)}")
     vocab, d = table.shape
@@ -210,6 +222,10 @@ def _ops_for(t, ops, what):
 
 # ---------------------------------------------------------------------------------------------------------------- Hugging Face LMs
 def _runs_here(t):
+    """libofhip takes this table, in plain or reverse-mode execution; everything else (forward-mode AD and torch.func's transforms among it)
+    keeps the LM's own modules, which support it"""
+    if _forward_mode() or torch._C._are_functorch_transforms_active():
+        return False
     try:
         helpers._require_hip(t, "vocabulary table")
     except (RuntimeError, TypeError):

@@ -1,0 +1,45 @@
+"""Calls of the vocabulary table's operators that the documentation allows and ordinary batches do not make, on the host emulator."""
+import types
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from open_flamingo_amd.train import vocab as V
+from tests import vocab_reference as R
+from tests.emu import harness
+
+
+@pytest.mark.parametrize("grads", [True, False])
+def test_forward_mode_is_refused_and_no_tangent_dropped(grads):
+    x, w, y = R.ce_inputs(3, 64, 20)
+    some = torch.tensor([3, 19, -100])
+    table, ids = torch.randn(5, 8, generator=torch.Generator().manual_seed(0)), torch.tensor([1, 4, 4])
+    plain = V.linear_cross_entropy(x, w, some, ops=harness.emu_ops()), V.embedding_lookup(ids, table, ops=harness.emu_ops())
+    with torch.set_grad_enabled(grads), forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))          # noqa: E731
+        for call in (lambda: V.linear_cross_entropy(dual(x), w, y, ops=harness.emu_ops()), lambda: V.linear_cross_entropy(x, dual(w), y, ops=harness.emu_ops()),
+                     lambda: V.embedding_lookup(ids, dual(table), ops=harness.emu_ops())):
+            with pytest.raises(NotImplementedError):
+                call()
+        # operands without a tangent are as before
+        assert torch.equal(V.linear_cross_entropy(x, w, some, ops=harness.emu_ops()), plain[0]) and torch.isfinite(plain[0])
+        assert torch.equal(V.embedding_lookup(ids, table, ops=harness.emu_ops()), plain[1])
+
+
+def test_the_lm_s_own_modules_serve_forward_mode_and_function_transforms(monkeypatch):
+    monkeypatch.setattr(V.helpers, "_require_hip", lambda t, what: None)
+    monkeypatch.setattr(V.Ops, "default", staticmethod(harness.emu_ops))
+    emb = torch.nn.Embedding(5, 8)
+    emb._of_eager_forward = emb.forward
+    emb.forward = types.MethodType(V._embedding_forward, emb)
+    ids, w = torch.tensor([[0, 4, 4]]), emb.weight.detach()
+    through = lambda t: torch.func.functional_call(emb, {"weight": t}, (ids,))          # noqa: E731
+    with forward_ad.dual_level():
+        tangent = forward_ad.unpack_dual(through(forward_ad.make_dual(w, 2 * w))).tangent
+    assert torch.equal(tangent, 2 * w[ids])
+    assert torch.equal(torch.func.jvp(through, (w,), (2 * w,))[1], 2 * w[ids])
+    want = torch.zeros(5, 8).index_add_(0, ids[0], torch.ones(3, 8))
+    assert torch.equal(torch.func.grad(lambda t: through(t).sum())(w), want)
+    emb(ids).sum().backward()          # outside of both: the operator and its own gradient
+    assert torch.equal(emb.weight.grad, want) and type(emb(ids).grad_fn).__name__.startswith(("_EmbeddingLookup", "View"))
