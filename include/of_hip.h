@@ -433,7 +433,8 @@ int of_embedding_bwd(const long long* ids, long n, const void* dy, int f32, long
  * OF_ADAMW_BLOCK consecutive elements of the tensor (ceil(n / 256) of them): first moment = code * scale, SQUARE ROOT of the second
  * moment = code * scale.  All-zero codes and scales are a fresh state.  The first moment is rounded to the nearest code, the root of the
  * second at random in proportion (a hash of tensor's place in the list, element and step: the same call gives the same bits).
- *   max_norm <= 0: no clipping.  *sumsq receives the squared norm.  A norm that is not finite leaves p, m, v and scales untouched.
+ *   max_norm <= 0: no clipping.  *sumsq receives the squared norm.  One that is not finite in fp32 (NaN, infinity, a norm
+ *   above 1.7e19: the squared gradients would not fit the moments) leaves p, m, v and scales untouched, with a clip too.
  *   step: 1-based; with applied_steps (device int) the count of applied updates there is advanced and used instead.
  * Workspace: of_adamw_multi_workspace_bytes(n), 16-byte aligned.  Tensors must not overlap. */
 #define OF_ADAMW_BLOCK 256

@@ -32,7 +32,7 @@ struct MtTensor {
 };
 // what the step's launches share, on the device
 struct MtStep {
-    float coef;                             // gradient factor of the clip; negative: a norm that is not finite, the step is left out
+    float coef;                             // gradient factor of the clip; negative: a squared norm that is not finite, the step is left out
     float inv_sqrt_bc2, inv_bc1;
     int t;
 };
@@ -167,7 +167,9 @@ OF_GLOBAL void OF_BOUNDS(256, 1) mt_begin_kernel(MtBeginArgs a) {
     s = mt_sum64(s, red, tid);
     if (tid == 0) {
         const float sum = (float)s, norm = (float)sqrt(s);
-        const bool finite = norm < 3.0e38f;
+        // the SQUARED norm has to be an fp32 value: no element's second moment then leaves the range (one that did would make its block's
+        // scale infinite, and with it every 8-bit code of the block NaN), and the caller sees from *sumsq that the step was left out
+        const bool finite = sum < 3.0e38f;
         *a.sumsq = sum;
         int t = a.step;
         if (a.applied) {

@@ -413,7 +413,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=0, lr=1e-3, betas=(
     device, none overlapping another.  lr, weight_decay: one value, or one per tensor.  max_norm <= 0: no clipping.
 
     step: 1-based count of this update; ``applied``, a device int32 counter, replaces it, and counts the updates that were applied.  A
-    gradient norm that is not finite leaves everything untouched (no host synchronisation).  May be captured into a graph: a replay keeps
+    squared gradient norm that is not finite in fp32 (a norm above 1.7e19 included, clipped or not) leaves everything untouched (no host
+    synchronisation; the returned value tells).  May be captured into a graph: a replay keeps
     the tensors' addresses, lr, weight_decay and step (give ``applied`` there).  Returns the squared norm (1, fp32)."""
     n = len(params)
     coded = exp_avg_scales is not None or exp_avg_sq_scales is not None
@@ -473,7 +474,7 @@ def _capturing():
 class MultiTensorAdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` for fp32 parameters through ``adamw_step``: every ``step()`` is one call over all parameters that have a gradient,
     whatever they are (a fully trained vocabulary table included, which ``FlatAdamW`` refuses), with ``clip_grad_norm_(max_norm)`` in it and no
-    host synchronisation; a gradient norm that is not finite skips the step.
+    host synchronisation; a gradient whose squared norm is not finite in fp32 (a norm above 1.7e19) skips the step.
 
     state_bits = 8 holds the moments in 2 bytes an element instead of 8 (see ``adamw_step``).  Groups have their own ``lr`` and
     ``weight_decay``; betas and eps are common to all (a group of its own values raises).  One count of applied updates serves all parameters
