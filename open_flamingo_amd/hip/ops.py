@@ -461,7 +461,9 @@ class Ops:
         if labels.dtype is not torch.int64 or not labels.is_contiguous() or labels.numel() != rows:
             raise ValueError("labels: one int64 per row, contiguous")
         assert cx == 1 and cw == 1
-        a = abi.OfLinearCeArgs(x=x.data_ptr(), ldx=max(ldx, d), w=w.data_ptr(), ldw=max(ldw, d), labels=labels.data_ptr(), ignore_index=ignore_index, rows=rows,
+        # (a matrix of one row may come with any stride and still be "contiguous": no address is formed from it)
+        ldx, ldw = max(ldx, d) if rows > 1 else d, max(ldw, d) if w.shape[0] > 1 else d
+        a = abi.OfLinearCeArgs(x=x.data_ptr(), ldx=ldx, w=w.data_ptr(), ldw=ldw, labels=labels.data_ptr(), ignore_index=ignore_index, rows=rows,
                                vocab=w.shape[0], d=d, logit_scale=logit_scale, reduction=reduction, piece=piece, early_dx=early)
         return a
 
@@ -495,10 +497,10 @@ class Ops:
         a.state, a.state_bytes, a.grad = state.data_ptr(), state.numel(), grad.data_ptr()
         if dx is not None:
             assert dx.dtype is BF16 and dx.shape == x.shape and dx.stride(1) == 1
-            a.dx, a.lddx = dx.data_ptr(), max(dx.stride(0), a.d)
+            a.dx, a.lddx = dx.data_ptr(), max(dx.stride(0), a.d) if dx.shape[0] > 1 else a.d
         if dw is not None:
             assert dw.dtype is BF16 and dw.shape == w.shape and dw.stride(1) == 1
-            a.dw, a.lddw = dw.data_ptr(), max(dw.stride(0), a.d)
+            a.dw, a.lddw = dw.data_ptr(), max(dw.stride(0), a.d) if dw.shape[0] > 1 else a.d
         ws = self._linear_ce_workspace(a, 1, x.device)          # noqa: F841
         self._chk(self.lib.of_linear_ce_bwd(a, self._stream()), "of_linear_ce_bwd")
 

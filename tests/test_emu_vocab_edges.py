@@ -43,3 +43,25 @@ def test_the_lm_s_own_modules_serve_forward_mode_and_function_transforms(monkeyp
     assert torch.equal(torch.func.grad(lambda t: through(t).sum())(w), want)
     emb(ids).sum().backward()          # outside of both: the operator and its own gradient
     assert torch.equal(emb.weight.grad, want) and type(emb(ids).grad_fn).__name__.startswith(("_EmbeddingLookup", "View"))
+
+
+@pytest.mark.parametrize("table_grad", [None, False, True])          # None: no gradient at all
+@pytest.mark.parametrize("rows,vocab", [(1, 30), (3, 1), (1, 1)])
+def test_matrices_of_one_row_with_any_stride(rows, vocab, table_grad):
+    """torch calls a matrix of one row contiguous whatever its row stride is"""
+    x, w, _ = R.ce_inputs(rows, 64, vocab, drop=0.0)
+    y = torch.arange(rows) % vocab
+    one = lambda t, stride: t if t.shape[0] > 1 else torch.nn.functional.pad(t, (0, stride - 64)).as_strided(t.shape, (stride, 1))          # noqa: E731
+
+    def run(x, w):
+        x, w = x.detach().requires_grad_(table_grad is not None), w.detach().requires_grad_(bool(table_grad))
+        loss = V.linear_cross_entropy(x, w, y, ops=harness.emu_ops())
+        if table_grad is None:
+            return loss.detach(), None, None
+        loss.backward()
+        return loss.detach(), x.grad, w.grad
+
+    want = run(x, w)
+    for stride in (65, 72, 1000001):
+        got = run(one(x, stride), one(w, stride))
+        assert all(a is None and b is None or torch.equal(a, b) for a, b in zip(got, want)), stride
