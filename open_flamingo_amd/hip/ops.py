@@ -510,7 +510,7 @@ class Ops:
         n, (vocab, d) = ids.numel(), table.shape
         assert ids.dtype is torch.int64 and ids.dim() == 1 and ids.is_contiguous() and out.dtype is table.dtype and out.shape == (n, d)
         (ldt, ct), (ldy, cy) = table.stride(), out.stride()
-        assert ct == 1 and cy == 1
+        assert d == 1 or (ct == 1 and cy == 1)          # (one column: its stride forms no address)
         rc = self.lib.of_embedding_fwd(ids.data_ptr(), n, table.data_ptr(), _is_f32(table), max(ldt, d), vocab, d, scale, out.data_ptr(), max(ldy, d),
                                        self._stream_fn())
         if rc:
@@ -521,7 +521,7 @@ class Ops:
         n, (vocab, d) = ids.numel(), dw.shape
         assert ids.dtype is torch.int64 and ids.dim() == 1 and ids.is_contiguous() and dy.dtype is dw.dtype and dy.shape == (n, d)
         (ldy, cy), (ldw, cw) = dy.stride(), dw.stride()
-        assert cy == 1 and cw == 1
+        assert d == 1 or (cy == 1 and cw == 1)
         size = self.lib.of_embedding_bwd_workspace_bytes(n, vocab, d)
         ws = torch.empty(size, dtype=torch.uint8, device=dw.device) if size else None
         rc = self.lib.of_embedding_bwd(ids.data_ptr(), n, dy.data_ptr(), _is_f32(dy), max(ldy, d), vocab, d, scale, padding_idx,

@@ -65,3 +65,17 @@ def test_matrices_of_one_row_with_any_stride(rows, vocab, table_grad):
     for stride in (65, 72, 1000001):
         got = run(one(x, stride), one(w, stride))
         assert all(a is None and b is None or torch.equal(a, b) for a, b in zip(got, want)), stride
+
+
+@pytest.mark.parametrize("vocab,ids", [(7, [1, 4, 4]), (7, [6]), (1, [0]), (1, [0, 0]), (300, list(range(0, 300, 3)))])
+def test_a_table_of_one_column_with_any_stride(vocab, ids):
+    """torch calls a matrix of one column contiguous whatever its column stride is; the gradient of a sum has none at all"""
+    ids, k = torch.tensor(ids), len(ids)
+    values = torch.arange(1.0, vocab + 1)
+    for table in (values[None].t(), values[:, None].clone(), values.repeat_interleave(3).as_strided((vocab, 1), (3, 7))):
+        for grad in (torch.ones(()).expand(k, 1), torch.ones(1, k).t(), torch.ones(k, 3)[:, :1]):
+            t = table.detach().requires_grad_()
+            y = V.embedding_lookup(ids, t, scale=2.0, ops=harness.emu_ops())
+            assert torch.equal(y.detach(), 2.0 * values[ids][:, None])
+            dt = torch.autograd.grad(y, t, grad)[0]
+            assert torch.equal(dt[:, 0], 2.0 * torch.bincount(ids, minlength=vocab).float())
