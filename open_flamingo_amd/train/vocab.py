@@ -127,7 +127,7 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
     y = labels if len(shape) == 2 and labels.is_contiguous() else labels.reshape(-1).contiguous()
     if n == 0:          # no rows: torch's values, zero gradients
         zero = (hidden.sum() + table[:0].sum()).to(F32)
-        return zero.new_zeros(labels.shape) if reduction == "none" else zero / 0.0 if reduction == "mean" else zero
+        return zero.expand(labels.shape) if reduction == "none" else zero / 0.0 if reduction == "mean" else zero
     kw = dict(ignore_index=int(ignore_index), logit_scale=float(logit_scale), reduction=_REDUCTION[reduction], piece=int(piece))
     other = _elsewhere(x)
     if other is None:

@@ -79,3 +79,18 @@ def test_a_table_of_one_column_with_any_stride(vocab, ids):
             assert torch.equal(y.detach(), 2.0 * values[ids][:, None])
             dt = torch.autograd.grad(y, t, grad)[0]
             assert torch.equal(dt[:, 0], 2.0 * torch.bincount(ids, minlength=vocab).float())
+
+
+@pytest.mark.parametrize("shape", [(0,), (0, 5), (2, 0)])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_no_rows_have_torch_s_values_and_zero_gradients(reduction, shape):
+    x, w = torch.zeros(*shape, 64).bfloat16().requires_grad_(), torch.ones(30, 64).bfloat16().requires_grad_()
+    y = torch.zeros(shape, dtype=torch.int64)
+    loss = V.linear_cross_entropy(x, w, y, reduction=reduction, ops=harness.emu_ops())
+    want = torch.nn.functional.cross_entropy(torch.zeros(0, 30), y.reshape(-1), reduction=reduction)
+    assert loss.dtype == want.dtype and loss.shape == (shape if reduction == "none" else ())
+    assert torch.equal(loss.detach().isnan().reshape(-1), want.isnan().reshape(-1)) and (loss.isnan() | (loss == 0)).all()
+    loss.sum().backward()
+    assert x.grad.shape == x.shape and w.grad.dtype == w.dtype and (w.grad == 0).all()
+    with torch.no_grad():
+        assert not V.linear_cross_entropy(x, w, y, reduction=reduction, ops=harness.emu_ops()).requires_grad
