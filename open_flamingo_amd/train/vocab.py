@@ -105,8 +105,8 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
         raise ValueError(f"labels {tuple(labels.shape)} do not fit hidden states {tuple(shape)}")
     if table.dim() != 2 or table.shape[1] != d or table.shape[0] == 0:
         raise ValueError(f"table {tuple(table.shape)} does not fit hidden states {tuple(shape)}")
-    if (n + 255) // 256 * 256 * ((d + 63) // 64 * 64) >= 1 << 31:
-        raise ValueError(f"{n} rows of {d}: the hidden states of a call must stay below 2^31 elements; split the batch")
+    if (n + 255) // 256 * 256 * max((d + 63) // 64 * 64, 256) >= 1 << 31:          # (256 table rows of logits gradient are the least a piece holds)
+        raise ValueError(f"{n} rows of {d}: a call must stay below 2^31 elements of hidden states and below 2^23 rows; split the batch")
     if d % 8:
         raise ValueError(f"the hidden size must be a multiple of 8, got {d}")
     if labels.dtype is not torch.int64:

@@ -94,3 +94,10 @@ def test_no_rows_have_torch_s_values_and_zero_gradients(reduction, shape):
     assert x.grad.shape == x.shape and w.grad.dtype == w.dtype and (w.grad == 0).all()
     with torch.no_grad():
         assert not V.linear_cross_entropy(x, w, y, reduction=reduction, ops=harness.emu_ops()).requires_grad
+
+
+@pytest.mark.parametrize("rows,d", [(2 ** 23 - 255, 8), (2 ** 23 - 255, 128), (2 ** 23, 64), (2 ** 19 - 255, 4096)])
+def test_batches_beyond_32_bit_offsets_are_refused_by_name(rows, d):
+    x, y = torch.zeros(1, d).bfloat16().expand(rows, d), torch.zeros(1, dtype=torch.int64).expand(rows)
+    with pytest.raises(ValueError, match="split the batch"):
+        V.linear_cross_entropy(x, torch.zeros(3, d).bfloat16(), y, ops=harness.emu_ops())
