@@ -5,6 +5,7 @@ Both are plain functions on tensors (``embedding_lookup``, ``linear_cross_entrop
 through them.  They stand beside ``towers.use_libofhip_lm_loss``, which computes the same loss from materialised logits, and
 ``sparse_rows``, which trains two rows of a frozen table.  GPU tensors only, like everything that runs on libofhip.
 """
+import threading
 import types
 
 import torch
@@ -268,8 +269,9 @@ class _VocabLossMixin:
             return super().forward(*args, **kwargs)
         labels = kwargs.pop("labels")
         kwargs.pop("logits_to_keep", None)
-        seen = []
-        hook = self.base_model.register_forward_hook(lambda mod, args, out: seen.append(out[0]))
+        seen, me = [], threading.get_ident()
+        # (the hook sits on a module that other threads may be running as well)
+        hook = self.base_model.register_forward_hook(lambda mod, args, out: seen.append(out[0]) if threading.get_ident() == me else None)
         try:          # the LM's own forward with no position for the head: hidden states, cache and all the rest as it makes them
             none = torch.empty(0, dtype=torch.int64, device=labels.device)
             out = super().forward(*args, logits_to_keep=none, **kwargs)
