@@ -409,8 +409,6 @@ OF_DEV unsigned of_f32_to_fp8x4(f32x4 v) {
 OF_DEV bool of_wave_any(bool p) { return __builtin_amdgcn_ballot_w64(p) != 0; }
 // 1-ulp hardware reciprocal (v_rcp_f32) instead of the ~12-instruction IEEE division sequence
 OF_DEV float of_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
-// 1-ulp hardware square root (v_sqrt_f32; values below the normal range count as zero)
-OF_DEV float of_sqrt(float x) { return __builtin_amdgcn_sqrtf(x); }
 // the value of lane `src` (wave-uniform) in a scalar register
 OF_DEV unsigned of_readlane(unsigned v, int src) { return (unsigned)__builtin_amdgcn_readlane((int)v, src); }
 typedef __bf16 of_bf16x2n __attribute__((ext_vector_type(2)));

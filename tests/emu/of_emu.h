@@ -393,7 +393,6 @@ OF_DEV void of_atomic_add(float* p, float v) {
 }
 OF_DEV float of_exp(float x) { return expf(x); }
 OF_DEV float of_rcp(float x) { return 1.0f / x; }
-OF_DEV float of_sqrt(float x) { return sqrtf(x); }
 OF_DEV unsigned of_readlane(unsigned v, int src) { return (unsigned)of_emu_bits(of_shfl(of_emu_float(v), src)); }
 OF_DEV float of_erf(float x) { return erff(x); }
 OF_DEV float of_tanh(float x) { return tanhf(x); }
