@@ -261,8 +261,7 @@ class _VocabLossMixin:
         if any(kwargs.get(k) is not None for k in ("num_items_in_batch", "shift_labels", "ignore_index")) or getattr(w, "_of_trained_rows", None) is not None:
             return False
         dev = w.device.type
-        amp = torch.is_autocast_enabled(dev) and torch.get_autocast_dtype(dev) == BF16
-        return amp or w.dtype == BF16
+        return (torch.get_autocast_dtype(dev) if torch.is_autocast_enabled(dev) else w.dtype) == BF16          # what the head would multiply in
 
     def forward(self, *args, **kwargs):
         if not self._of_takes(args, kwargs):
