@@ -238,6 +238,13 @@ def _keeps_all(logits_to_keep):
     return isinstance(logits_to_keep, int) and logits_to_keep == 0
 
 
+def _plain_product(head):
+    """The head is x @ weight.T and nothing besides: no bias, no forward of its own (an adapter's, a patched one), no hooks that would see or change
+    the logits."""
+    return (isinstance(head, torch.nn.Linear) and type(head).forward is torch.nn.Linear.forward and "forward" not in head.__dict__ and head.bias is None
+            and not (head._forward_hooks or head._forward_pre_hooks or head._backward_hooks or head._backward_pre_hooks))
+
+
 def _embedding_forward(self, ids):
     if ids.dtype == torch.int64 and self.weight.dtype in (F32, BF16) and _runs_here(self.weight):
         return embedding_lookup(ids, self.weight, padding_idx=self.padding_idx)
@@ -247,7 +254,7 @@ def _embedding_forward(self, ids):
 class _VocabLossMixin:
     """``forward(labels=...)`` of a Hugging Face causal LM without logits: the output's ``loss`` comes from ``linear_cross_entropy`` on the
     last hidden states and the head's weight, its ``logits`` is None.  Without labels nothing changes.  What the operator does not
-    cover (a head with a bias, ``logits_to_keep``, other loss arguments, operands that are not bf16 or under bf16 autocast, the two-row mode of
+    cover (a head with a bias, hooks or a forward of its own, ``logits_to_keep``, other loss arguments, operands that are not bf16 or under bf16 autocast, the two-row mode of
     train/sparse_rows.py, whose tap sits behind the logits) takes the LM's own path."""
 
     def _of_takes(self, args, kwargs):
@@ -256,7 +263,7 @@ class _VocabLossMixin:
             return False
         head = self.get_output_embeddings()
         w = getattr(head, "weight", None)
-        if labels is None or w is None or w.shape[1] % 8 or getattr(head, "bias", None) is not None or not _keeps_all(kwargs.get("logits_to_keep", 0)) or not _runs_here(w):
+        if labels is None or w is None or w.shape[1] % 8 or not _plain_product(head) or not _keeps_all(kwargs.get("logits_to_keep", 0)) or not _runs_here(w):
             return False
         if any(kwargs.get(k) is not None for k in ("num_items_in_batch", "shift_labels", "ignore_index")) or getattr(w, "_of_trained_rows", None) is not None:
             return False

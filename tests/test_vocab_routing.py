@@ -53,3 +53,33 @@ def test_autocast_decides_the_heads_type_and_so_the_route(route):
         assert route(half) == route(full) == "operator"
     with torch.autocast("cpu", dtype=torch.float16):          # the LM's own head multiplies in fp16 here, also where its weight is bf16
         assert route(half) == route(full) == "own"
+
+
+def test_a_head_that_does_more_than_multiply_is_not_passed_by(route):
+    class Scaled(torch.nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Adapter(torch.nn.Module):          # a wrapper that shows its base's weight
+        def __init__(self, base):
+            super().__init__()
+            self.base = base
+
+        weight = property(lambda self: self.base.weight)
+        bias = property(lambda self: self.base.bias)
+
+        def forward(self, x):
+            return self.base(x) + 1
+
+    plain = torch.nn.Linear(8, 10, bias=False)
+    patched, hooked, before = (torch.nn.Linear(8, 10, bias=False) for _ in range(3))
+    patched.forward = lambda x: x @ patched.weight.t() * 3
+    hook = hooked.register_forward_hook(lambda mod, args, out: out + 1)
+    before.register_forward_pre_hook(lambda mod, args: (args[0] * 2,))
+    tied = torch.nn.utils.parametrize.register_parametrization(torch.nn.Linear(8, 10, bias=False), "weight", torch.nn.Identity())
+    want = [(plain, "operator"), (tied, "operator"), (Scaled(8, 10, bias=False), "own"), (Adapter(torch.nn.Linear(8, 10, bias=False)), "own"), (patched, "own"),
+            (hooked, "own"), (before, "own"), (torch.nn.Linear(8, 10), "own")]
+    for i, (head, path) in enumerate(want):
+        assert route(V.use_libofhip_vocab(MptForCausalLM(head).bfloat16())) == path, i
+    hook.remove()          # without it the head is a plain product again
+    assert route(V.use_libofhip_vocab(MptForCausalLM(hooked).bfloat16())) == "operator"
