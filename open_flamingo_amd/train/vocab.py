@@ -300,7 +300,7 @@ def use_libofhip_vocab(lm):
     if isinstance(lm, _VocabLossMixin):
         return lm
     emb = lm.get_input_embeddings()
-    if type(emb) is torch.nn.Embedding and emb.max_norm is None and not emb.scale_grad_by_freq and not emb.sparse:
+    if type(emb) is torch.nn.Embedding and "forward" not in emb.__dict__ and emb.max_norm is None and not emb.scale_grad_by_freq and not emb.sparse:
         emb._of_eager_forward = emb.forward
         emb.forward = types.MethodType(_embedding_forward, emb)
     extend_instance(lm, _VocabLossMixin)

@@ -83,3 +83,17 @@ def test_a_head_that_does_more_than_multiply_is_not_passed_by(route):
         assert route(V.use_libofhip_vocab(MptForCausalLM(head).bfloat16())) == path, i
     hook.remove()          # without it the head is a plain product again
     assert route(V.use_libofhip_vocab(MptForCausalLM(hooked).bfloat16())) == "operator"
+
+
+def test_a_lookup_that_was_patched_before_stays(route):
+    lm = MptForCausalLM()
+    own = lm.transformer.wte.forward
+    lm.transformer.wte.forward = lambda ids: 2 * own(ids)
+    ids = torch.tensor([[1, 2]])
+    assert torch.equal(V.use_libofhip_vocab(lm).transformer.wte(ids), 2 * lm.transformer.wte.weight[ids])
+    first = V.use_libofhip_vocab(MptForCausalLM())
+    third = MptForCausalLM()
+    third.transformer.wte = first.transformer.wte          # a table of two LMs, routed by both
+    V.use_libofhip_vocab(third)
+    half = third.half().transformer.wte          # a type the operator does not take: the module's own lookup
+    assert torch.equal(half(ids), half.weight[ids])
