@@ -20,6 +20,9 @@ SOURCES = ["gemm.hip", "gemm_pp.hip", "gemm_w4.hip", "gemm_w4m.hip", "gemm_w4h.h
 HEADERS = ["of_platform.h", "gemm_common.h", "gemm_tile256.h", "gemm_w4_epi.h", "gemm_ce_epi.h", "attn_core.h", os.path.join(ROOT, "include", "of_hip.h")]
 # kernels of_gemm never selects (measured, kept with their tests and records): tools / emulator builds only, not in the product library
 TOOLS_ONLY_SOURCES = ["gemm_w4.hip", "gemm_w4s.hip"]
+FLAGS = ["--offload-arch=gfx950", "-std=c++17", "-O3", "-fPIC", "-I", HERE,
+         "-Wno-unused-function", "-fno-fast-math",   # erf / tanh / division semantics of the epilogues stay IEEE
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]   # no v_pk_{add,mul,fma}_f32: some forms of them have returned wrong values
 LIB = os.path.join(HERE, "libofhip.so")
 EMU_DIR = os.path.join(ROOT, "tests", "emu")
 EMU_LIB = os.path.join(EMU_DIR, "libofhip_emu.so")
@@ -54,9 +57,7 @@ def build(emu=False, verbose=False, force=False, tools=False):
         link = ["/opt/rocm/lib/llvm/bin/clang++", "-shared", "-pthread"]
     else:
         objdir = os.path.join(HERE, "build_tools" if tools else "build")
-        cc = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-std=c++17", "-O3", "-fPIC", "-I", HERE,
-              "-Wno-unused-function", "-fno-fast-math",   # erf / tanh / division semantics of the epilogues stay IEEE
-              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]   # no v_pk_{add,mul,fma}_f32: some forms of them have returned wrong values
+        cc = ["/opt/rocm/bin/hipcc"] + FLAGS
         if tools:
             cc.append("-DOF_TOOLS_BUILD")
         lib = TOOLS_LIB if tools else LIB
