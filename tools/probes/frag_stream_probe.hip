@@ -8,7 +8,7 @@
 //   2  bpermute: row-major, coalesced quads (lane l: row l >> 2, chunk l & 3) + 4 ds_bpermute_b32 into the fragment layout
 //   3  packed + no MFMA (fetch only: the L2 -> CU ceiling)
 // Shapes: "q" = N 512 x K 2048 (wave w owns n-tiles 4w..4w+3, 64 k-steps), "o" = N 2048 x K 512 (wave w owns 16 n-tiles, 16 k-steps).
-// Build: hipcc --offload-arch=gfx950 -O3 tools/probes/frag_stream_probe.hip -o tools/probes/frag_stream_probe
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probes/frag_stream_probe.hip -o tools/probes/frag_stream_probe
 // PROFILING TOOL, not part of the library.
 #include <hip/hip_runtime.h>
 #include <cstdio>

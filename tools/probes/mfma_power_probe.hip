@@ -1,6 +1,6 @@
 // MFMA-only probe (gfx950): the same FLOPs through v_mfma_f32_32x32x16_bf16 and v_mfma_f32_16x16x32_bf16, one wave per SIMD,
 // 256 accumulator registers, random bf16 operands held in registers -- what the power-limited clock gives each instruction
-// shape.  Build: hipcc --offload-arch=gfx950 -O3 tools/probes/mfma_power_probe.hip -o tools/probes/mfma_power_probe
+// shape.  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probes/mfma_power_probe.hip -o tools/probes/mfma_power_probe
 // PROFILING TOOL, not part of the library.
 #include <hip/hip_runtime.h>
 #include <cstdio>
