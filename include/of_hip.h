@@ -384,6 +384,8 @@ int of_ce_bwd(const void* logits, int logits_f32, long ld, const long long* labe
  *              early_dx = 1 (dx wanted, dw not: a frozen table; the same in forward and backward): the forward sums dx as well, in `state`, from
  *              the one logits product, and the backward only finishes it.
  *              of_linear_ce_stateless(rows, d) = 1 (a handful of rows: scoring next tokens): `state` may be NULL, with no backward to follow
+ * The logits' gradient is rounded to bf16 between the products (half a step, 2^-8 of an entry), statistics and sums are fp32.  Rows rounded up
+ * to 256 times d rounded up to 64 (at least 256) stay below 2^31 (OF_E_SHAPE otherwise).
  * Deterministic: no atomics.  d % 8 == 0; x, w, dx, dw 16-byte aligned like state and workspace, row strides
  * multiples of 8.  The workspace holds of_linear_ce_workspace_bytes(args, backward) bytes: the fields rows, vocab, d, ldw, piece, early_dx,
  * reduction, state and (backward) dx of args decide. */

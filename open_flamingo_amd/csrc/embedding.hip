@@ -1,8 +1,8 @@
 // Lookup in a vocabulary table with a scale, and its gradient by sorted tokens (gfx950, HBM-bound).
 //   y[i] = scale * W[id_i]                       one wave per position, 16-byte loads and stores
 //   dW[v] = scale * sum over {i: id_i = v} dy[i]   in fp32, positions in ascending order; rows without a token are zeros
-// The gradient has to read dy once (n x d) and to write the table once (vocabulary x d); torch scatters with atomics into a zeroed
-// table and rounds behind every addition where the table is bf16.  Here, without floating-point atomics:
+// The gradient has to read dy once (n x d) and to write the table once (vocabulary x d).  Scattered with atomics into a zeroed table it would
+// depend on their order, and round behind every addition where the table is bf16.  Here, without floating-point atomics:
 //   sort     (id, position) by id, stable: radix passes of 9 bits.  Up to 16384 positions ONE workgroup sorts in LDS while the
 //            others of the same launch clear the table; more positions take two launches a pass (counts, placement), from 2^22 + 1 on a
 //            third that adds the counts up.
@@ -12,8 +12,9 @@
 //            partial rows in the workspace;
 //   join     the chunk in which a crossing token begins adds the partial rows of the chunks behind it, in order.
 // The same ids and gradients give the same bits on every run.
-// Measured: 8192 tokens of a 50435 x 2048 fp32 table, forward and gradient 134 us (lookup 38, sort beside the clearing of 413 MB 58, sums 32, join
-// 5; 614 MB); 32768 tokens, 4096 columns of bf16, skewed ids: 306 us (lookup 89, the rest 218).
+// Measured: 8192 tokens of a 50435 x 2048 fp32 table, forward and gradient 134 us (lookup 39, sort beside the clearing of 413 MB 58, sums 33, join
+// 5; 614 MB); 32768 tokens, 4096 columns of bf16, skewed ids: 309 us (lookup 85, the rest 222).  Waited for one by one 181 and 347 us; torch's
+// embedding module takes 323 and 1310 (the second with its scaling as a pass of its own), and 34 and 93 against 36 and 100 forward alone.
 #include "gemm_common.h"
 
 namespace {
@@ -113,8 +114,8 @@ OF_DEV void emb_scan_bins(int* cum, int tid) {
     }
 }
 
-// Turns cnt[wave][digit] (how often each wave met each digit) into the place of the wave's first such element: in a tile of its own
-// (base = nullptr), or behind base[digit * stride].  The waves hold consecutive parts of the tile: the order stays.  LDS: cnt, cum[BINS];
+// Turns cnt[wave][digit] (how often each wave met each digit) into the place of the wave's first such element: in a tile that is all there
+// is (given = false), or from `at`, the place of the tile's first element of digit `tid`.  The waves hold consecutive parts of the tile: the order stays.  LDS: cnt, cum[BINS];
 // every thread of the workgroup calls.
 template <class CNT>
 OF_DEV void emb_offsets(CNT* cnt, int* cum, int waves, int tid, bool given, int at) {
@@ -590,8 +591,8 @@ extern "C" int of_embedding_bwd(const long long* ids, long n, const void* dy, in
             a.key_out = key[0]; a.pos_out = pos[0];
             a.cap = (int)(n + 63) / 64 * 64;
             const size_t lds = 2 * (size_t)a.cap * 4 + SMALL_WAVES * BINS * 2 + BINS * 4;
-            // 256 workgroups sweep the table in windows of 4 MB: 766 MB cleared beside a sort of 39 positions takes 138 us in all; 255, 511
-            // and 1022 of them, whose windows do not end at a power of two, take 166, 155 and 170, 512 (two to a compute unit) 159
+            // 256 workgroups sweep the table in windows of 4 MB: the gradient of 65 positions of a 766-MB table takes 139 us (a fill alone 113);
+            // 255, 511 and 1022 of them, whose windows do not end at a power of two, take 167, 156 and 169, 512 (two to a compute unit) 159
             rc = of_launch(emb_sort_small_kernel, of_dim3{(unsigned)(1 + (fill < 256 ? fill : 256)), 1, 1}, SMALL_THREADS, lds, s, a);
             if (rc) return rc;
         } else {

@@ -5,16 +5,18 @@
 // to 8 bits of mantissa in front of the exponential.  Here:
 //   forward   rows whose label counts are gathered (an ignored row costs nothing behind this point), then ONE product whose epilogue
 //             keeps (max, sum exp) per row and 128 columns, from fp32 accumulators; a small launch joins the ~400 strips of a row;
-//   backward  the vocabulary in pieces: the product again -> D of the piece (bf16, at most a few hundred MB, sized so that it stays in
-//             the 256-MB Infinity Cache between the three products that touch it) -> dx += D W_piece in fp32, dW_piece = D^T x.
+//   backward  the vocabulary in pieces: the product again -> D of the piece (bf16; 128 MB, so that it stays in the 256-MB Infinity Cache
+//             between the three products that touch it; never under 256 table rows, i.e. 512 bytes a row of the batch: 512 MB at 2^20
+//             rows) -> dx += D W_piece in fp32, dW_piece = D^T x.
 //   frozen table   without dW the forward forms dx as well and the backward has no product left (two instead of three): E = exp(z - c) with
 //             c = the label's logit needs no maximum, dx = s g (exp(c - lse) E W + (p_label - 1) w_label).  lse - c is the row's loss; only a
 //             loss above 80 (in units of log 2) could overflow, and then a flag on the device lets the forms above run behind it.
 // All products run on the 256x256 MFMA kernel (gemm_w4m.hip) with the epilogues of gemm_ce_epi.h: they are bound by its K loop, i.e. by
 // the chip's power budget, 2 R V d operations forward and 6 R V d backward (a third of them the second logits product).
-// Measured (8192 rows, 9 of 10 count, d = 2048, vocabulary 50435): loss and both gradients 5.00 ms = four products of 1.52 TFLOP at 1217
-// TFLOP/s (1.18 ms statistics, 1.40 logits again, 1.42 dx, 1.24 dW; a library product of that shape reaches 1282), 66 us in the small
-// launches; d = 4096 9.90 ms, 1299 TFLOP/s.  Frozen table, 1999 rows (half count), d = 2560: 0.56 ms.  One row: 47 us, 207 MB at 4.8 TB/s.
+// Measured (8192 rows, 7361 count, d = 2048, vocabulary 50435; kernel times and calls of one profiled run): loss and both gradients 4.97 ms =
+// four products of 1.52 TFLOP at 1235 TFLOP/s (1.10 ms statistics, 1.31 logits again, 1.34 dx, 1.18 dW; a library product of that shape reaches
+// 1282) and 60 us in the small launches; d = 4096, 9 of 10 and more count: 9.88 ms, 1310 TFLOP/s.  Frozen table, 1999 rows (1013 count), d = 2560:
+// 0.56 ms (0.26 EARLY, 0.26 dx); 1032 that count are a fifth tile of rows: 0.66.  One row: 47 us, 207 MB at 4.8 TB/s.
 // No atomics; every sum has a fixed order.
 #include "gemm_ce_epi.h"
 

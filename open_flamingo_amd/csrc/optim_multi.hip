@@ -7,11 +7,16 @@
 // moments = 3.84 GB at 5.05 TB/s, a large copy's rate (update 620, norm 125 us); 492 us with 8-bit moments = 2.40 GB at 4.9 TB/s.
 //
 // 8-bit moments: e4m3 codes with one fp32 scale (largest magnitude / 448) per 256 consecutive elements of a tensor.
-//   * The first moment is rounded to the nearest code: it moves by a tenth of its distance to g' every step, more than half a code.
+//   * The first moment is rounded to the nearest code: it moves by a tenth of its distance to g' every step, and stands still where that is
+//     less than half a code (1/32 ... 1/16 of it), i.e. within 0.3 ... 0.6 of it from g'.
 //   * The second moment is held as its square root, which halves the range of exponents a code has to cover.  It moves by a thousandth
-//     (b2 = 0.999) of its distance to g'^2 a step, far less than half a code (1/16 ... 1/32): rounded to the nearest it would stand
-//     still.  It is rounded up or down at random in proportion, so that its expectation is exact; the 20 random bits are a hash of (tensor,
-//     element, step): the same call gives the same bits.  From above zero it never goes to zero (m / (0 + eps) would explode).
+//     (b2 = 0.999) of its distance to g'^2 a step, far less than half a code: rounded to the nearest it would stand still.  It is rounded up
+//     or down at random in proportion, so that the ROOT's expectation is the unrounded one's (the second moment itself gains the rounding's
+//     variance); the 20 random bits are a hash of (tensor, element, step): the same call gives the same bits.  From above zero it never goes
+//     to zero (m / (0 + eps) would explode).
+//   * What that comes to beside 32 bits, 1000 to 20000 steps of noisy gradients of a fixed mean (8192 elements, b = 0.9, 0.999): the second
+//     moment 3 to 7 % high, its root between -24 % and +31 % (5th to 95th percentile), the first moment 4 to 5 % off (rms); the sum of the
+//     updates has a cosine of 0.994 and more with that of 32 bits and is 1 % longer.  None of it grows with the steps.
 //   * The parameter's own update uses the moments in fp32, before they are rounded.
 #include "of_platform.h"
 #include "../../include/of_hip.h"

@@ -409,7 +409,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=0, lr=1e-3, betas=(
 
     params: fp32; grads: fp32 or bf16 (left as they are); exp_avgs, exp_avg_sqs: fp32, or -- with ``exp_avg_scales`` and
     ``exp_avg_sq_scales`` -- 8-bit codes (torch.float8_e4m3fn) of the first moment and of the SQUARE ROOT of the second, one fp32 scale
-    per 256 consecutive elements (value = code * scale; zeros are a fresh state; ``adamw_state`` makes them).  All contiguous, on one
+    per 256 consecutive elements (value = code * scale; zeros are a fresh state).  All contiguous, on one
     device, none overlapping another.  lr, weight_decay: one value, or one per tensor.  max_norm <= 0: no clipping.
 
     step: 1-based count of this update; ``applied``, a device int32 counter, replaces it, and counts the updates that were applied.  A
@@ -476,7 +476,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     whatever they are (a fully trained vocabulary table included, which ``FlatAdamW`` refuses), with ``clip_grad_norm_(max_norm)`` in it and no
     host synchronisation; a gradient whose squared norm is not finite in fp32 (a norm above 1.7e19) skips the step.
 
-    state_bits = 8 holds the moments in 2 bytes an element instead of 8 (see ``adamw_step``).  Groups have their own ``lr`` and
+    state_bits = 8 holds the moments in 2 bytes an element instead of 8 (see ``adamw_step``), and is not the 32-bit update: over thousands of
+    steps the second moment is about 5 % high, its root scatters by a quarter to a third around the 32-bit one, the first moment is off by 4 to
+    5 % and stands still within 0.3 to 0.6 of itself from the gradient; the sum of the updates kept a cosine of 0.99 with 32 bits'.  Groups have their own ``lr`` and
     ``weight_decay``; betas and eps are common to all (a group of its own values raises).  One count of applied updates serves all parameters
     (torch keeps one each: the same unless a parameter goes without a gradient for some steps).  ``state_dict`` has torch.optim.AdamW's layout
     for 32 bits; for 8 bits ``exp_avg`` and ``exp_avg_sq`` hold codes beside ``exp_avg_scale`` and ``exp_avg_sq_scale``."""

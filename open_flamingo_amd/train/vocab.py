@@ -97,8 +97,12 @@ def linear_cross_entropy(hidden, table, labels, *, ignore_index=-100, reduction=
     hidden (..., d) and table (vocabulary, d): bfloat16, or any floating type under bf16 autocast (cast as ``F.linear`` casts); d a
     multiple of 8.  labels (...): int64, already shifted.  reduction "mean" (over the labels that count: NaN without any), "sum" or
     "none" (one fp32 loss per label, 0 where ignored).  A label outside the vocabulary that is not ``ignore_index`` makes the loss NaN and
-    has no gradient.  Where the table has no gradient the forward prepares the hidden states' one from the same product.  Gradients come in bfloat16 for both operands, through fp32 sums; ``piece``: vocabulary rows the backward
-    holds a logits gradient of at a time (0: chosen, 128 MB of it).  Differentiable once, backward; forward-mode AD raises."""
+    has no gradient.
+
+    Gradients come in bfloat16 for both operands, through fp32 sums of products whose one factor, the logits' gradient (softmax - onehot,
+    or exp(logit - label's logit) where the table has no gradient), is rounded to bfloat16: half a step, 2^-8 of each entry, on the way.
+    Where the table has no gradient the forward prepares the hidden states' one from the same product.  ``piece``: vocabulary rows the
+    backward holds a logits gradient of at a time (0: chosen, 128 MB of it).  Differentiable once, backward; forward-mode AD raises."""
     if reduction not in _REDUCTION:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {reduction!r}")
     shape, d, n = hidden.shape, hidden.shape[-1], labels.numel()
